@@ -495,7 +495,7 @@ int srbcrs_group_norm_backward(const srbcrs_norm_desc *desc, const void *d_dy, c
  * has a loss of 0, does not count in the mean and gets a gradient of 0; a
  * target outside [0, classes) that is not ignore_index gives a loss of NaN.
  * reduction: NONE writes `rows` floats to d_loss, MEAN (over the labelled
- * rows; 0 if there is none) and SUM one.  d_state, 2 * rows + 3 floats (8-byte
+ * rows; 0 if there is none) and SUM one.  d_state, 2 * rows + 1 floats (8-byte
  * aligned), is kept from the forward pass for the backward pass. */
 #define SRBCRS_REDUCE_NONE 0
 #define SRBCRS_REDUCE_MEAN 1

@@ -5,7 +5,7 @@
 // Operand rows.  An operand is rows of 128-byte steps, 128-byte aligned or at
 // least 16-byte aligned.  kF16 / kBf16: a step is 64 values.  kSplit: a step
 // is 32 values of a 32-bit matrix, each as the sum of two float16, 64 bytes of
-// high parts and then 64 bytes of low parts.  With the matrix scaled by a
+// high parts and then 64 bytes of low parts.  With a row, or the matrix, scaled by a
 // power of two to a largest value in [2^14, 2^15), high + low hold 22 bits of every
 // value down to 2^-29 of the largest, and an absolute error of 2^-40 of it
 // below.  A product of two such matrices is

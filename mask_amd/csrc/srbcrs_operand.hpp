@@ -1,10 +1,12 @@
 // Operand rows for the dense products (srbcrs_dense.hpp) from a caller's
-// matrix: its rows, or its columns, scaled by a power of two, whole steps of
-// 128 bytes with zeros past the last value.
+// matrix, whole steps of 128 bytes with zeros past the last value.
 //
-// The power of two comes from the largest finite magnitude, kept as the bits of a float in an
-// unsigned (atomicMax over non-negative floats: the order does not matter).
-// A matrix of zeros, or with none finite, is scaled by 1.
+// Its rows: 16 bits as they are; 32 bits each scaled by a power of two of its own, from its largest
+// finite magnitude, so that no row's values cost another row's digits; its inverse's exponent
+// goes to the product's end.
+// Its columns: scaled by one power of two, from the largest finite magnitude of the matrix, kept as the bits of a float
+// in an unsigned (atomicMax over non-negative floats: the order does not matter).
+// What is all zeros, or has none finite, is scaled by 1.
 #pragma once
 #include "srbcrs_dense.hpp"
 #include "srbcrs_ops.h"
@@ -12,13 +14,13 @@
 namespace srbcrs {
 namespace dense {
 
-// 2^(14 - exponent): the largest magnitude lands in [2^14, 2^15).
-__device__ __forceinline__ float scale_of(const unsigned* max_bits) {
-  const unsigned b = *max_bits;
-  const int e = (int)(b >> 23) - 127;
-  // clamped: the scale and its inverse are normal floats
-  return b == 0 ? 1.f : __builtin_bit_cast(float, (unsigned)(min(max(14 - e, -126), 126) + 127) << 23);
+// 14 - exponent: scaled by 2 to its power, the largest magnitude lands in [2^14, 2^15).
+// Clamped: the scale and its inverse are normal floats.
+__device__ __forceinline__ int scale_exponent(unsigned max_bits) {
+  return max_bits == 0 ? 0 : min(max(14 - ((int)(max_bits >> 23) - 127), -126), 126);
 }
+__device__ __forceinline__ float power_of_two(int e) { return __builtin_bit_cast(float, (unsigned)(e + 127) << 23); }
+__device__ __forceinline__ float scale_of(const unsigned* max_bits) { return power_of_two(scale_exponent(*max_bits)); }
 __device__ __forceinline__ float inverse_scale(const unsigned* max_bits) {
   const unsigned s = __builtin_bit_cast(unsigned, scale_of(max_bits));
   return __builtin_bit_cast(float, (254u - (s >> 23)) << 23);
@@ -53,7 +55,8 @@ struct Source {
   int64_t ld, rows, cols;
   char* dst;                     // operand rows
   int64_t ld_dst;
-  unsigned* max_bits;            // its largest magnitude, null: not scaled
+  int* exponent;                 // of each row, of its scale's inverse (k_pack_rows)
+  unsigned* max_bits;            // its largest magnitude, null: not scaled (k_pack_t)
   const float* factor;           // of its rows (k_pack_t), null: none
   const unsigned* factor_max;
 };
@@ -112,14 +115,13 @@ __global__ __launch_bounds__(1024) void k_absmax(Pair<T> pair) {
   join_max(m, src.max_bits);
 }
 
-// Rows: dst row r holds x[r][:] * scale.  Four values a thread, four times in flight.
+// Rows of 16 bits: dst row r holds x[r][:].  Four values a thread, four times in flight.
 template <int KIND, class T>
 __global__ __launch_bounds__(256) void k_pack(Pair<T> pair) {
   const Source<T>& src = pair.m[blockIdx.y];
   const T* x = src.x;
   const int64_t ld = src.ld, rows = src.rows, cols = src.cols, ld_dst = src.ld_dst;
   char* dst = src.dst;
-  const float scale = src.max_bits ? scale_of(src.max_bits) : 1.f;
   const int64_t quads = ld_dst / kStep * (step_values(KIND) / 4), n = rows * quads, all = (int64_t)gridDim.x * 256;
   const bool narrow = n < (1ll << 31);   // a 64-bit division takes longer than the copy
   typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
@@ -145,7 +147,61 @@ __global__ __launch_bounds__(256) void k_pack(Pair<T> pair) {
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (i0 + u * all < n) put4<KIND>(dst + r[u] * ld_dst, c[u], v[u] * scale);
+      if (i0 + u * all < n) put4<KIND>(dst + r[u] * ld_dst, c[u], v[u]);
+  }
+}
+
+// Rows of 32 bits, each with its own scale: `lanes` lanes a row, a power of two that is at most a wave, four quads of
+// values a lane in flight.  Rows of up to 1024 values stay in registers between their maximum and
+// their place; longer ones are read again, from the cache that they have just passed.
+template <class T>
+__global__ __launch_bounds__(256) void k_pack_rows(Pair<T> pair, int lanes) {
+  const Source<T>& src = pair.m[blockIdx.y];
+  const int cols = (int)src.cols, quads = (int)(src.ld_dst / kStep * (step_values(kSplit) / 4));
+  const int lane = threadIdx.x & (lanes - 1), per_block = 256 / lanes;
+  typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  constexpr int U = 4;
+  for (int64_t r = (int64_t)blockIdx.x * per_block + threadIdx.x / lanes; r < src.rows; r += (int64_t)gridDim.x * per_block) {
+    const T* x = src.x + r * src.ld;
+    char* to = src.dst + r * src.ld_dst;
+    float4v v[U];
+    auto load = [&](int q0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int q = q0 + u * lanes, c = 4 * q;
+        v[u] = float4v{0.f, 0.f, 0.f, 0.f};
+        if (c + 4 <= cols) {
+          const vec t = *(const vec*)(x + c);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[u][e] = (float)t[e];
+        } else if (c < cols) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[u][e] = c + e < cols ? (float)x[c + e] : 0.f;
+        }
+      }
+    };
+    float m = 0.f;
+    for (int q0 = lane; q0 < quads; q0 += U * lanes) {
+      load(q0);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float a = fabsf(v[u][e]);
+          m = a < INFINITY ? fmaxf(m, a) : m;
+        }
+    }
+    for (int d = lanes / 2; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+    const int e = scale_exponent(__builtin_bit_cast(unsigned, m));
+    const float scale = power_of_two(e);
+    if (lane == 0) src.exponent[r] = -e;
+    const bool held = quads <= U * lanes;
+    for (int q0 = lane; q0 < quads; q0 += U * lanes) {
+      if (!held) load(q0);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (q0 + u * lanes < quads) put4<kSplit>(to, 4 * (q0 + u * lanes), v[u] * scale);
+    }
   }
 }
 
@@ -226,6 +282,16 @@ void pack(const Pair<T>& p, int n, hipStream_t s) {
     most = most > quads ? most : quads;
   }
   k_pack<KIND, T><<<dim3(blocks_for(most, 256 * 4, 8192), n), 256, 0, s>>>(p);
+}
+// rows of one length
+template <class T>
+void pack_rows(const Pair<T>& p, int n, hipStream_t s) {
+  const int64_t quads = p.m[0].ld_dst / kStep * (step_values(kSplit) / 4);
+  int lanes = 1;
+  while (lanes < 64 && lanes < quads) lanes *= 2;
+  int64_t most = 0;
+  for (int i = 0; i < n; ++i) most = most > p.m[i].rows ? most : p.m[i].rows;
+  k_pack_rows<T><<<dim3(blocks_for(most, 256 / lanes, 8192), n), 256, 0, s>>>(p, lanes);
 }
 // the rows of dst reach to whole steps: tiles of 64 rows of x cover them
 template <int KIND, class T>

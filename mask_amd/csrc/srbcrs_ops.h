@@ -36,7 +36,6 @@ struct XentArgs {
   int reduction;             // 0 none, 1 mean, 2 sum
   float* lse;                // rows: kept from the forward pass for the backward pass
   float* count;              // 1: max(labelled rows, 1), likewise
-  unsigned* maxima;          // 2: of h and w, likewise (32-bit inputs)
   void* ws;
 };
 // ws == null: nothing runs.  Returns the bytes of workspace that the call uses.

@@ -195,7 +195,6 @@ int srbcrs_linear_xent(const srbcrs_xent_desc* desc, const void* d_h, const void
     check_aligned(d_weight, a.dtype, "weight");
     check_ws(d_ws, ws_bytes, xent_forward(a, nullptr, nullptr));
     a.target = d_target, a.lse = d_state, a.count = d_state + 2 * a.rows, a.ws = d_ws;
-    a.maxima = (unsigned*)a.count + 1;
     xent_forward(a, d_loss, (hipStream_t)stream);
     check_launches("linear cross entropy");
   });
@@ -221,7 +220,6 @@ int srbcrs_linear_xent_backward(const srbcrs_xent_desc* desc, const void* d_h, c
     for (const void* p : {d_h, d_weight, (const void*)d_dh, (const void*)d_dweight}) check_aligned(p, a.dtype, "a matrix");
     check_ws(d_ws, ws_bytes, xent_backward(a, nullptr, d_dh, d_dweight, nullptr));
     a.target = d_target, a.lse = (float*)d_state, a.count = (float*)d_state + 2 * a.rows, a.ws = d_ws;
-    a.maxima = (unsigned*)a.count + 1;
     xent_backward(a, d_dloss, d_dh, d_dweight, (hipStream_t)stream);
     check_launches("linear cross entropy's backward pass");
   });

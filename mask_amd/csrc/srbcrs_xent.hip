@@ -29,28 +29,45 @@ constexpr int64_t kPieceBytes = 512ll << 20;
 // Largest magnitudes of h, w and the rows' factors.
 struct Scalars { unsigned *hmax, *wmax, *gmax; };
 
+// Exponents of what a product of scaled rows lacks, of every row of w and of h; null: rows are as they are.
+// Both reach to a whole number of tiles (what is past the last row is not used).
+struct Exponents {
+  const int *w, *h;
+  // of four rows of w
+  __device__ __forceinline__ int4 of_w(int v) const { return w ? *(const int4*)(w + v) : make_int4(0, 0, 0, 0); }
+  __device__ __forceinline__ int of_h(int t) const { return h ? h[t] : 0; }
+};
+__device__ __forceinline__ float4v logits_of(float4v sum, int4 ew, int eh) {
+  return float4v{__builtin_amdgcn_ldexpf(sum[0], ew.x + eh), __builtin_amdgcn_ldexpf(sum[1], ew.y + eh),
+                 __builtin_amdgcn_ldexpf(sum[2], ew.z + eh), __builtin_amdgcn_ldexpf(sum[3], ew.w + eh)};
+}
+
 // unnormalised row statistics: the largest logit and the sum of exp(z - it)
 struct StatEpi : WaveEpi {
-  const unsigned *hmax, *wmax;   // null: operands not scaled
+  Exponents ex;
   float2* part;                  // [parts][rows]
   float* zt;
   const int64_t* target;
   int rows, classes;
   template <int TI, int TJ>
   __device__ void store(float4v (&acc)[TI][TJ], const Where& w) const {
-    const float scale = (hmax ? inverse_scale(hmax) : 1.f) * (wmax ? inverse_scale(wmax) : 1.f);
+    int4 ew[TI];
+#pragma unroll
+    for (int i = 0; i < TI; ++i) ew[i] = ex.of_w(row_of(w, i));
 #pragma unroll
     for (int j = 0; j < TJ; ++j) {
-      const int t = col_of(w, j);
+      const int t = col_of(w, j), eh = ex.of_h(t);
       float mx = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < TI; ++i)
+      for (int i = 0; i < TI; ++i) {
+        acc[i][j] = logits_of(acc[i][j], ew[i], eh);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float z = row_of(w, i) + e < classes ? acc[i][j][e] * scale : -INFINITY;
+          const float z = row_of(w, i) + e < classes ? acc[i][j][e] : -INFINITY;
           acc[i][j][e] = z;
           mx = fmaxf(mx, z);
         }
+      }
       mx = fmaxf(mx, __shfl_xor(mx, 16));
       mx = fmaxf(mx, __shfl_xor(mx, 32));
       const float ref = mx == -INFINITY ? 0.f : mx;
@@ -78,7 +95,7 @@ struct StatEpi : WaveEpi {
 
 template <int KIND>   // of dz
 struct GradEpi : WaveEpi {
-  const unsigned *hmax, *wmax;
+  Exponents ex;
   const float2* lse;             // row: largest logit, 1 / sum of exponentials
   const int64_t* target;
   int64_t ignore;
@@ -87,7 +104,6 @@ struct GradEpi : WaveEpi {
   int rows, classes, first;      // first: the piece's first class
   template <int TI, int TJ>
   __device__ void store(float4v (&acc)[TI][TJ], const Where& w) const {
-    const float scale = (hmax ? inverse_scale(hmax) : 1.f) * (wmax ? inverse_scale(wmax) : 1.f);
     constexpr int SV = step_values(KIND);
     const int classes_up = (classes + SV - 1) / SV * SV, rows_up = (rows + SV - 1) / SV * SV;
     // the statistics of this lane's columns: rows of h
@@ -102,6 +118,13 @@ struct GradEpi : WaveEpi {
       st[j] = live[j] ? lse[t] : make_float2(0.f, 0.f);
       at[j] = tg >= first && tg < (int64_t)first + classes ? (int)(tg - first) : -1;
     }
+    if (ex.w)
+#pragma unroll
+      for (int i = 0; i < TI; ++i) {
+        const int4 ew = ex.of_w(row_of(w, i));
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) acc[i][j] = logits_of(acc[i][j], ew, ex.of_h(col_of(w, j)));
+      }
     through_lds<TI, TJ>(
         acc, w,
         [&](int v, int t, float4v z) {
@@ -109,7 +132,7 @@ struct GradEpi : WaveEpi {
           float4v d;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float p = __builtin_amdgcn_exp2f((z[e] * scale - st[j].x) * kLog2e) * st[j].y;
+            float p = __builtin_amdgcn_exp2f((z[e] - st[j].x) * kLog2e) * st[j].y;
             p = v + e == at[j] ? p - 1.f : p;
             d[e] = live[j] && v + e < classes ? p * kDzScale : 0.f;
           }
@@ -270,15 +293,18 @@ bool usable(const void* p, int64_t ld, int64_t dim) {
 struct Logits {
   Operand w, h;
   int kind;
-  const unsigned *hmax = nullptr, *wmax = nullptr;
-  Logits(const XentArgs& a, Carver& c, const Scalars& sc, hipStream_t s) {
+  Exponents ex{};
+  Logits(const XentArgs& a, Carver& c, hipStream_t s) {
     kind = a.dtype == kF32T ? kSplit : a.dtype == kBf16T ? kBf16 : kF16;
     const bool go = a.ws != nullptr;
-    if (kind == kSplit) hmax = sc.hmax, wmax = sc.wmax;
     // {weight, features}: as they are, or copies
     const void* p[2] = {a.w, a.h};
     const int64_t ld[2] = {a.ldw, a.ldh}, rows[2] = {a.classes, a.rows}, rb = row_bytes(kind, a.dim);
-    const unsigned* mx[2] = {wmax, hmax};
+    int* exponent[2] = {};
+    if (kind == kSplit) {
+      for (int i = 0; i < 2; ++i) exponent[i] = c.take<int>(round_up(rows[i], tile_size(kTile256)));
+      ex = {exponent[0], exponent[1]};
+    }
     Operand o[2];
     int copied[2], n = 0;
     for (int i = 0; i < 2; ++i) {
@@ -294,9 +320,10 @@ struct Logits {
       Pair<T> pair{};
       for (int k = 0; k < n; ++k) {
         const int i = copied[k];
-        pair.m[k] = {(const T*)p[i], ld[i], rows[i], a.dim, (char*)o[i].p, rb, (unsigned*)mx[i], nullptr, nullptr};
+        pair.m[k] = {(const T*)p[i], ld[i], rows[i], a.dim, (char*)o[i].p, rb, exponent[i], nullptr, nullptr, nullptr};
       }
-      pack<decltype(kind_c)::value>(pair, n, s);
+      if constexpr (decltype(kind_c)::value == kSplit) pack_rows(pair, n, s);
+      else pack<decltype(kind_c)::value>(pair, n, s);
     };
     if (go && n) {
       if (kind == kSplit) copy(std::integral_constant<int, kSplit>{}, (const float*)nullptr);
@@ -343,8 +370,8 @@ void backward_pieces(const XentArgs& a, Carver& c, const Logits& lg, const Scala
       using T = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
       Pair<T> pair{};
       int n = 0;
-      if (dh) pair.m[n++] = {(const T*)a.w, a.ldw, a.classes, a.dim, wt, ldw, (unsigned*)wmax, nullptr, nullptr};
-      if (dw) pair.m[n++] = {(const T*)a.h, a.ldh, a.rows, a.dim, ht, ldh, (unsigned*)hmax, factor, sc.gmax};
+      if (dh) pair.m[n++] = {(const T*)a.w, a.ldw, a.classes, a.dim, wt, ldw, nullptr, (unsigned*)wmax, nullptr, nullptr};
+      if (dw) pair.m[n++] = {(const T*)a.h, a.ldh, a.rows, a.dim, ht, ldh, nullptr, (unsigned*)hmax, factor, sc.gmax};
       pack_t<KIND>(pair, n, s);
     };
     if constexpr (KIND == kSplit) turn((const float*)nullptr);
@@ -362,7 +389,7 @@ void backward_pieces(const XentArgs& a, Carver& c, const Logits& lg, const Scala
       Operand wp = lg.w;
       wp.p = (const char*)wp.p + v0 * wp.ld;
       wp.rows = (int)n;
-      GradEpi<KIND> e{{}, lg.hmax, lg.wmax, (const float2*)a.lse, a.target, a.ignore, dz, dzt, ldz, ldzt,
+      GradEpi<KIND> e{{}, {lg.ex.w ? lg.ex.w + v0 : nullptr, lg.ex.h}, (const float2*)a.lse, a.target, a.ignore, dz, dzt, ldz, ldzt,
                       (int)a.rows, (int)n, (int)v0};
       lg.run<KIND == kSplit, true>(cut, wp, a.dim, e, scratch, s);
     }
@@ -392,8 +419,8 @@ void maxima(const XentArgs& a, const Scalars& sc, hipStream_t s) {
   auto both = [&](auto* t) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
     Pair<T> pair{};
-    pair.m[0] = {(const T*)a.w, a.ldw, a.classes, a.dim, nullptr, 0, sc.wmax, nullptr, nullptr};
-    pair.m[1] = {(const T*)a.h, a.ldh, a.rows, a.dim, nullptr, 0, sc.hmax, nullptr, nullptr};
+    pair.m[0] = {(const T*)a.w, a.ldw, a.classes, a.dim, nullptr, 0, nullptr, sc.wmax, nullptr, nullptr};
+    pair.m[1] = {(const T*)a.h, a.ldh, a.rows, a.dim, nullptr, 0, nullptr, sc.hmax, nullptr, nullptr};
     absmax(pair, 2, s);
   };
   if (a.dtype == kF32T) both((const float*)nullptr);
@@ -426,7 +453,6 @@ size_t xent_forward(const XentArgs& a, float* loss, hipStream_t s) {
   if (few_forwards(a, usable(a.h, a.ldh, a.dim) && usable(a.w, a.ldw, a.dim))) return few_forward(a, loss, s);
   const bool go = a.ws != nullptr;
   Carver c(a.ws);
-  const Scalars sc{a.maxima, a.maxima + 1, nullptr};   // the backward pass finds them there
   // statistics are per wave of a tile: no join from parts of the sum
   const Cut cut = cut_for(a.dtype == kF32T ? kSplit : kBf16, a.classes, a.rows, a.dim, 1, false, false);
   const int64_t parts = (a.classes + tile_size(cut.tile) - 1) / tile_size(cut.tile) * waves_m(cut.tile);
@@ -436,13 +462,9 @@ size_t xent_forward(const XentArgs& a, float* loss, hipStream_t s) {
   const bool wide = a.rows <= 256, some = a.rows <= 4096;
   const unsigned blocks = (unsigned)(wide ? a.rows : some ? (a.rows + 3) / 4 : (a.rows + 31) / 32);
   float2* bs = a.reduction ? c.take<float2>(blocks) : nullptr;
-  if (go && a.dtype == kF32T) {
-    k_zero_words<<<1, 64, 0, s>>>(a.maxima, 2);
-    maxima(a, sc, s);
-  }
-  Logits lg(a, c, sc, s);
+  const Logits lg(a, c, s);
   if (!go) return c.used;
-  const StatEpi epi{{}, lg.hmax, lg.wmax, part, zt, a.target, (int)a.rows, (int)a.classes};
+  const StatEpi epi{{}, lg.ex, part, zt, a.target, (int)a.rows, (int)a.classes};
   if (lg.kind == kSplit) lg.run<true, false>(cut, lg.w, a.dim, epi, nullptr, s);
   else lg.run<false, false>(cut, lg.w, a.dim, epi, nullptr, s);
   float* each = a.reduction ? nullptr : loss;
@@ -462,17 +484,15 @@ size_t xent_backward(const XentArgs& a, const float* dloss, void* dh, void* dw, 
   if (few_backwards(a)) return few_backward(a, dloss, dh, dw, s);
   const bool go = a.ws != nullptr;
   Carver c(a.ws);
-  // of 32-bit inputs the forward pass left the maxima
-  const bool known = a.dtype == kF32T;
-  unsigned* own = c.take<unsigned>(3);
-  const Scalars sc{known ? a.maxima : own, known ? a.maxima + 1 : own + 1, own + 2};
+  unsigned* words = c.take<unsigned>(3);
+  const Scalars sc{words, words + 1, words + 2};
   float* factor = c.take<float>(round_up(a.rows, 32));
   if (go) {
-    if (!known) k_zero_words<<<1, 64, 0, s>>>(own, 3);
-    factors(a, dloss, factor, sc.gmax, !known, s);
-    if (!known) maxima(a, sc, s);
+    k_zero_words<<<1, 64, 0, s>>>(words, 3);
+    factors(a, dloss, factor, sc.gmax, true, s);
+    maxima(a, sc, s);
   }
-  Logits lg(a, c, sc, s);
+  const Logits lg(a, c, s);
   size_t used = c.used;
   if (a.dtype == kF32T) backward_pieces<kSplit>(a, c, lg, sc, factor, dh, dw, s, used);
   else backward_pieces<kF16>(a, c, lg, sc, factor, dh, dw, s, used);

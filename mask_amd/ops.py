@@ -237,7 +237,7 @@ def _xent_forward(h, weight, target, ignore, reduction):
         desc, n = _xent_plan(h, weight, ignore, reduction, 0)
         rows = h.shape[0]
         loss = torch.empty((rows,) if reduction == 0 else (), dtype=torch.float32, device=h.device)
-        state = torch.empty(2 * rows + 3, dtype=torch.float32, device=h.device)
+        state = torch.empty(2 * rows + 1, dtype=torch.float32, device=h.device)
         ws = _workspace(n, h)
         _capi.check(_capi.lib().srbcrs_linear_xent(
             desc, h.data_ptr(), weight.data_ptr(), target.data_ptr(), loss.data_ptr(), state.data_ptr(), _capi.ptr(ws), n,
