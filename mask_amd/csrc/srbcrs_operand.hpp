@@ -4,9 +4,12 @@
 // Its rows: 16 bits as they are; 32 bits each scaled by a power of two of its own, from its largest
 // finite magnitude, so that no row's values cost another row's digits; its inverse's exponent
 // goes to the product's end.
-// Its columns: scaled by one power of two, from the largest finite magnitude of the matrix, kept as the bits of a float
-// in an unsigned (atomicMax over non-negative floats: the order does not matter).
+// Its columns: their sum runs over the rows, so one power of two scales all of them, from the largest finite magnitude
+// of a row times the row's factor: rows that do not count (factor 0) have no say in it.
 // What is all zeros, or has none finite, is scaled by 1.
+//
+// Maxima of many workgroups are joined by atomicMax on unsigned (of floats that are not negative the bits):
+// the order does not matter.
 #pragma once
 #include "srbcrs_dense.hpp"
 #include "srbcrs_ops.h"
@@ -20,10 +23,18 @@ __device__ __forceinline__ int scale_exponent(unsigned max_bits) {
   return max_bits == 0 ? 0 : min(max(14 - ((int)(max_bits >> 23) - 127), -126), 126);
 }
 __device__ __forceinline__ float power_of_two(int e) { return __builtin_bit_cast(float, (unsigned)(e + 127) << 23); }
-__device__ __forceinline__ float scale_of(const unsigned* max_bits) { return power_of_two(scale_exponent(*max_bits)); }
-__device__ __forceinline__ float inverse_scale(const unsigned* max_bits) {
-  const unsigned s = __builtin_bit_cast(unsigned, scale_of(max_bits));
-  return __builtin_bit_cast(float, (254u - (s >> 23)) << 23);
+
+// The largest factor's magnitude, 1 where all are 0.
+__device__ __forceinline__ float factor_unit(const unsigned* max_bits) {
+  return *max_bits ? __builtin_bit_cast(float, *max_bits) : 1.f;
+}
+// A magnitude's exponent, biased: 0 only of 0.  Products of two floats neither overflow nor vanish in 64 bits.
+__device__ __forceinline__ unsigned exponent_of(double v) { return v > 0. ? (unsigned)__double2hiint(v) >> 20 : 0u; }
+// Of a matrix whose entries times their factors have `largest` as their largest exponent_of, for
+// factors in units of the largest one (unit null: none): they land below 2^15.
+__device__ __forceinline__ int scale_exponent(const unsigned* largest, const unsigned* unit) {
+  const int u = unit ? (int)exponent_of(factor_unit(unit)) - 1023 : 0;
+  return *largest == 0 ? 0 : min(max(14 - ((int)*largest - 1023 - u), -126), 126);
 }
 
 template <class T>
@@ -34,16 +45,17 @@ __global__ __launch_bounds__(64) void k_zero_words(T* p, int n) {
 // A workgroup's maximum to *out: one atomic each, and at most a workgroup a CU, since
 // atomics on one word follow each other at about 10 ns (4096 of them cost 40 us).  A launch
 // of one workgroup sets *out, more of them need a zero there first.
-__device__ __forceinline__ void join_max(float m, unsigned* out) {
-  __shared__ float all[16];
+__device__ __forceinline__ void join_max(unsigned m, unsigned* out) {
+  __shared__ unsigned all[16];
 #pragma unroll
-  for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+  for (int d = 32; d; d >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, d));
+  __syncthreads();   // an earlier call's are read
   if ((threadIdx.x & 63) == 0) all[threadIdx.x >> 6] = m;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int i = 1; i < (int)(blockDim.x >> 6); ++i) m = fmaxf(m, all[i]);
-    if (gridDim.x == 1) *out = __builtin_bit_cast(unsigned, m);
-    else if (m > 0.f) atomicMax(out, __builtin_bit_cast(unsigned, m));
+    for (int i = 1; i < (int)(blockDim.x >> 6); ++i) m = max(m, all[i]);
+    if (gridDim.x == 1) *out = m;
+    else if (m) atomicMax(out, m);
   }
 }
 
@@ -56,8 +68,10 @@ struct Source {
   char* dst;                     // operand rows
   int64_t ld_dst;
   int* exponent;                 // of each row, of its scale's inverse (k_pack_rows)
-  unsigned* max_bits;            // its largest magnitude, null: not scaled (k_pack_t)
-  const float* factor;           // of its rows (k_pack_t), null: none
+  float* row_max;                // of each row, its largest finite magnitude (k_row_max, k_pack_rows), null: not wanted
+  // of k_pack_t
+  const unsigned* largest;       // exponent_of its entries times their factors, null: not scaled
+  const float* factor;           // of its rows, null: none
   const unsigned* factor_max;
 };
 template <class T>
@@ -103,16 +117,29 @@ __device__ __forceinline__ void walk(const T* x, int64_t ld, int64_t rows, int64
   }
 }
 
-// max over the finite |x[r][c]|
+// The largest finite |x[r][:]| of every row r, by `lanes` lanes a row (a power of two, a wave at most).
 template <class T>
-__global__ __launch_bounds__(1024) void k_absmax(Pair<T> pair) {
+__global__ __launch_bounds__(256) void k_row_max(Pair<T> pair, int lanes) {
   const Source<T>& src = pair.m[blockIdx.y];
-  float m = 0.f;
-  walk(src.x, src.ld, src.rows, src.cols, [&](float v) {
-    v = fabsf(v);
-    m = v < INFINITY ? fmaxf(m, v) : m;
-  });
-  join_max(m, src.max_bits);
+  const int cols = (int)src.cols, lane = threadIdx.x & (lanes - 1), per_block = 256 / lanes;
+  typedef T vec __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+  for (int64_t r = (int64_t)blockIdx.x * per_block + threadIdx.x / lanes; r < src.rows; r += (int64_t)gridDim.x * per_block) {
+    const T* x = src.x + r * src.ld;
+    float m = 0.f;
+    auto see = [&](float v) {
+      v = fabsf(v);
+      m = v < INFINITY ? fmaxf(m, v) : m;
+    };
+#pragma unroll 4
+    for (int c = 8 * lane; c + 8 <= cols; c += 8 * lanes) {
+      const vec v = *(const vec*)(x + c);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) see((float)v[e]);
+    }
+    for (int c = (cols & ~7) + lane; c < cols; c += lanes) see((float)x[c]);
+    for (int d = lanes / 2; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+    if (lane == 0) src.row_max[r] = m;
+  }
 }
 
 // Rows of 16 bits: dst row r holds x[r][:].  Four values a thread, four times in flight.
@@ -195,6 +222,7 @@ __global__ __launch_bounds__(256) void k_pack_rows(Pair<T> pair, int lanes) {
     const int e = scale_exponent(__builtin_bit_cast(unsigned, m));
     const float scale = power_of_two(e);
     if (lane == 0) src.exponent[r] = -e;
+    if (lane == 0 && src.row_max) src.row_max[r] = m;
     const bool held = quads <= U * lanes;
     for (int q0 = lane; q0 < quads; q0 += U * lanes) {
       if (!held) load(q0);
@@ -205,11 +233,6 @@ __global__ __launch_bounds__(256) void k_pack_rows(Pair<T> pair, int lanes) {
   }
 }
 
-// The largest factor's magnitude, 1 where all are 0.
-__device__ __forceinline__ float factor_unit(const unsigned* max_bits) {
-  return *max_bits ? __builtin_bit_cast(float, *max_bits) : 1.f;
-}
-
 // Columns: dst row c holds x[:][c] * scale (* factor[r] / the largest factor: exactly 1 where all
 // are the same; a zero factor gives a zero whatever x holds).  A workgroup turns a 64 x 64 tile in LDS.
 template <int KIND, class T>
@@ -218,10 +241,11 @@ __global__ __launch_bounds__(256) void k_pack_t(Pair<T> pair) {
   const T* x = src.x;
   const int64_t ld = src.ld, rows = src.rows, cols = src.cols, ld_dst = src.ld_dst;
   char* dst = src.dst;
-  const unsigned *max_bits = src.max_bits, *factor_max = src.factor_max;
+  const unsigned* factor_max = src.factor_max;
   const float* factor = src.factor;
   __shared__ float tile[64][65];
-  const float scale = max_bits ? scale_of(max_bits) : 1.f, unit = factor_max ? factor_unit(factor_max) : 1.f;
+  const float scale = src.largest ? power_of_two(scale_exponent(src.largest, factor_max)) : 1.f;
+  const float unit = factor_max ? factor_unit(factor_max) : 1.f;
   const int64_t ct = (cols + 63) / 64, c0 = (blockIdx.x % ct) * 64, r0 = (blockIdx.x / ct) * 64;
   if (r0 >= rows) return;   // the other matrix has more tiles
   typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
@@ -244,9 +268,10 @@ __global__ __launch_bounds__(256) void k_pack_t(Pair<T> pair) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int64_t r = r0 + ty + 16 * i;
-    const float f = factor && r < rows ? factor[r] / unit : 1.f;
+    // the scale first with the factor: a large value of a small factor does not overflow
+    const float f = factor && r < rows ? factor[r] / unit * scale : scale;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) tile[ty + 16 * i][tx + q] = f == 0.f ? 0.f : v[i][q] * scale * f;
+    for (int q = 0; q < 4; ++q) tile[ty + 16 * i][tx + q] = f == 0.f ? 0.f : v[i][q] * f;
   }
   __syncthreads();
   // 16 quads of 4 values along r for each of 64 columns
@@ -267,12 +292,20 @@ inline unsigned blocks_for(int64_t work, int64_t per_block, int64_t most = 4096)
   return (unsigned)(n < 1 ? 1 : n > most ? most : n);
 }
 
-// of n matrices (1 or 2)
+// lanes that share a row of `loads` loads
+inline int lanes_for(int64_t loads) {
+  int lanes = 1;
+  while (lanes < 64 && lanes < loads) lanes *= 2;
+  return lanes;
+}
 template <class T>
-void absmax(const Pair<T>& p, int n, hipStream_t s) {
-  int64_t most = 0;
-  for (int i = 0; i < n; ++i) most = most > p.m[i].rows * p.m[i].cols ? most : p.m[i].rows * p.m[i].cols;
-  k_absmax<T><<<dim3(blocks_for(most, 1024 * 16, 256), n), 1024, 0, s>>>(p);
+int64_t most_rows(const Pair<T>& p, int n) { return n > 1 && p.m[1].rows > p.m[0].rows ? p.m[1].rows : p.m[0].rows; }
+
+// of n matrices (1 or 2) of one width
+template <class T>
+void row_maxima(const Pair<T>& p, int n, hipStream_t s) {
+  const int lanes = lanes_for(p.m[0].cols / 8);
+  k_row_max<T><<<dim3(blocks_for(most_rows(p, n), 256 / lanes, 8192), n), 256, 0, s>>>(p, lanes);
 }
 template <int KIND, class T>
 void pack(const Pair<T>& p, int n, hipStream_t s) {
@@ -286,12 +319,8 @@ void pack(const Pair<T>& p, int n, hipStream_t s) {
 // rows of one length
 template <class T>
 void pack_rows(const Pair<T>& p, int n, hipStream_t s) {
-  const int64_t quads = p.m[0].ld_dst / kStep * (step_values(kSplit) / 4);
-  int lanes = 1;
-  while (lanes < 64 && lanes < quads) lanes *= 2;
-  int64_t most = 0;
-  for (int i = 0; i < n; ++i) most = most > p.m[i].rows ? most : p.m[i].rows;
-  k_pack_rows<T><<<dim3(blocks_for(most, 256 / lanes, 8192), n), 256, 0, s>>>(p, lanes);
+  const int lanes = lanes_for(p.m[0].ld_dst / kStep * (step_values(kSplit) / 4));
+  k_pack_rows<T><<<dim3(blocks_for(most_rows(p, n), 256 / lanes, 8192), n), 256, 0, s>>>(p, lanes);
 }
 // the rows of dst reach to whole steps: tiles of 64 rows of x cover them
 template <int KIND, class T>

@@ -26,8 +26,9 @@ constexpr float kDzScale = 16384.f;          // |softmax - onehot| <= 1 to float
 // 21 % with 100000 x 256 against 1000, both float32; twice as much gains the first 8 % and nothing else, for twice the memory.
 constexpr int64_t kPieceBytes = 512ll << 20;
 
-// Largest magnitudes of h, w and the rows' factors.
-struct Scalars { unsigned *hmax, *wmax, *gmax; };
+// What the backward pass's operands are scaled by: exponents of the largest h times its row's
+// factor and of the largest w (null: they are not scaled), and the largest factor.
+struct Scalars { unsigned *h_largest, *w_largest, *gmax; };
 
 // Exponents of what a product of scaled rows lacks, of every row of w and of h; null: rows are as they are.
 // Both reach to a whole number of tiles (what is past the last row is not used).
@@ -267,9 +268,15 @@ __global__ __launch_bounds__(1024) void k_xent_total(const float2* __restrict__ 
 __global__ __launch_bounds__(256) void k_xent_factor(const float* __restrict__ dloss, const int64_t* __restrict__ target,
                                                      int64_t ignore, int classes, const float* __restrict__ count,
                                                      int reduction, int64_t rows, int64_t rows_up, float* __restrict__ factor,
-                                                     unsigned* __restrict__ fmax) {
+                                                     unsigned* __restrict__ fmax, Magnitudes mag) {
   float m = 0.f;
+  unsigned largest = 0;
   const int64_t all = (int64_t)gridDim.x * 256;
+  if (blockIdx.y) {   // the weight's
+    for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < classes; v += all) m = fmaxf(m, mag.w[v]);
+    join_max(exponent_of(m), mag.w_largest);
+    return;
+  }
   for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < rows_up; t += all) {
     const int64_t tg = t < rows ? target[t] : ignore;
     float f = 0.f;
@@ -279,9 +286,13 @@ __global__ __launch_bounds__(256) void k_xent_factor(const float* __restrict__ d
     }
     factor[t] = f;
     const float af = fabsf(f);
-    if (af < INFINITY && af > m) m = af;
+    if (af < INFINITY) {
+      m = fmaxf(m, af);
+      if (mag.h && t < rows) largest = max(largest, exponent_of((double)mag.h[t] * af));
+    }
   }
-  join_max(m, fmax);
+  join_max(__builtin_bit_cast(unsigned, m), fmax);
+  if (mag.h) join_max(largest, mag.h_largest);
 }
 
 // Rows of 16-bit values that the products can read where they are.
@@ -294,12 +305,14 @@ struct Logits {
   Operand w, h;
   int kind;
   Exponents ex{};
-  Logits(const XentArgs& a, Carver& c, hipStream_t s) {
+  // row_max_w, row_max_h: rows' largest magnitudes, written where 32-bit rows are packed; null: not wanted
+  Logits(const XentArgs& a, Carver& c, hipStream_t s, float* row_max_w = nullptr, float* row_max_h = nullptr) {
     kind = a.dtype == kF32T ? kSplit : a.dtype == kBf16T ? kBf16 : kF16;
     const bool go = a.ws != nullptr;
     // {weight, features}: as they are, or copies
     const void* p[2] = {a.w, a.h};
     const int64_t ld[2] = {a.ldw, a.ldh}, rows[2] = {a.classes, a.rows}, rb = row_bytes(kind, a.dim);
+    float* row_max[2] = {row_max_w, row_max_h};
     int* exponent[2] = {};
     if (kind == kSplit) {
       for (int i = 0; i < 2; ++i) exponent[i] = c.take<int>(round_up(rows[i], tile_size(kTile256)));
@@ -320,7 +333,7 @@ struct Logits {
       Pair<T> pair{};
       for (int k = 0; k < n; ++k) {
         const int i = copied[k];
-        pair.m[k] = {(const T*)p[i], ld[i], rows[i], a.dim, (char*)o[i].p, rb, exponent[i], nullptr, nullptr, nullptr};
+        pair.m[k] = {(const T*)p[i], ld[i], rows[i], a.dim, (char*)o[i].p, rb, exponent[i], row_max[i], nullptr, nullptr, nullptr};
       }
       if constexpr (decltype(kind_c)::value == kSplit) pack_rows(pair, n, s);
       else pack<decltype(kind_c)::value>(pair, n, s);
@@ -356,8 +369,6 @@ void backward_pieces(const XentArgs& a, Carver& c, const Logits& lg, const Scala
   if (piece < 256) piece = 256;
   if (piece > a.classes) piece = a.classes;
   const int64_t n_pieces = (a.classes + piece - 1) / piece;
-  const bool scaled = a.dtype != kF16T;   // float16 inputs are operands as they are
-  const unsigned *hmax = scaled ? sc.hmax : nullptr, *wmax = scaled ? sc.wmax : nullptr;
   const int64_t ldw = row_bytes(KIND, a.classes), ldh = row_bytes(KIND, a.rows);
   char* wt = dh ? c.take<char>(a.dim * ldw) : nullptr;
   char* ht = dw ? c.take<char>(a.dim * ldh) : nullptr;
@@ -370,8 +381,8 @@ void backward_pieces(const XentArgs& a, Carver& c, const Logits& lg, const Scala
       using T = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
       Pair<T> pair{};
       int n = 0;
-      if (dh) pair.m[n++] = {(const T*)a.w, a.ldw, a.classes, a.dim, wt, ldw, nullptr, (unsigned*)wmax, nullptr, nullptr};
-      if (dw) pair.m[n++] = {(const T*)a.h, a.ldh, a.rows, a.dim, ht, ldh, nullptr, (unsigned*)hmax, factor, sc.gmax};
+      if (dh) pair.m[n++] = {(const T*)a.w, a.ldw, a.classes, a.dim, wt, ldw, nullptr, nullptr, sc.w_largest, nullptr, nullptr};
+      if (dw) pair.m[n++] = {(const T*)a.h, a.ldh, a.rows, a.dim, ht, ldh, nullptr, nullptr, sc.h_largest, factor, sc.gmax};
       pack_t<KIND>(pair, n, s);
     };
     if constexpr (KIND == kSplit) turn((const float*)nullptr);
@@ -396,7 +407,7 @@ void backward_pieces(const XentArgs& a, Carver& c, const Logits& lg, const Scala
     c.used = mark;
     if (dh) {
       const bool last = p + 1 == n_pieces;
-      Out o{last ? dh : sum, a.dim, last ? a.dtype : kF32T, p ? sum : nullptr, wmax, 1.f / kDzScale,
+      Out o{last ? dh : sum, a.dim, last ? a.dtype : kF32T, p ? sum : nullptr, sc.w_largest, 1.f / kDzScale,
             last ? factor : nullptr, nullptr, (int)a.rows, (int)a.dim};
       product<KIND>(Operand{dz, ldz, 0, (int)a.rows},
                     Operand{wt + v0 / step_values(KIND) * kStep, ldw, 0, (int)a.dim}, n, o, c, s, go);
@@ -404,7 +415,7 @@ void backward_pieces(const XentArgs& a, Carver& c, const Logits& lg, const Scala
       c.used = mark;
     }
     if (dw) {
-      Out o{(char*)dw + v0 * a.dim * dtype_size(a.dtype), a.dim, a.dtype, nullptr, hmax, 1.f / kDzScale,
+      Out o{(char*)dw + v0 * a.dim * dtype_size(a.dtype), a.dim, a.dtype, nullptr, sc.h_largest, 1.f / kDzScale,
             nullptr, sc.gmax, (int)n, (int)a.dim};
       product<KIND>(Operand{dzt, ldzt, 0, (int)n}, Operand{ht, ldh, 0, (int)a.dim}, a.rows, o, c, s, go);
       used = used > c.used ? used : c.used;
@@ -412,19 +423,6 @@ void backward_pieces(const XentArgs& a, Carver& c, const Logits& lg, const Scala
     }
   }
   used = used > c.used ? used : c.used;
-}
-
-// float16 inputs are operands as they are
-void maxima(const XentArgs& a, const Scalars& sc, hipStream_t s) {
-  auto both = [&](auto* t) {
-    using T = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
-    Pair<T> pair{};
-    pair.m[0] = {(const T*)a.w, a.ldw, a.classes, a.dim, nullptr, 0, nullptr, sc.wmax, nullptr, nullptr};
-    pair.m[1] = {(const T*)a.h, a.ldh, a.rows, a.dim, nullptr, 0, nullptr, sc.hmax, nullptr, nullptr};
-    absmax(pair, 2, s);
-  };
-  if (a.dtype == kF32T) both((const float*)nullptr);
-  else if (a.dtype == kBf16T) both((const __bf16*)nullptr);
 }
 
 void join_parts(const float* part, int splits, const Out& o, hipStream_t s) {
@@ -438,11 +436,12 @@ void join_stats(const float2* part, int parts, const float* zt, const XentArgs& 
 void total(const float2* block_sum, int n, const XentArgs& a, float* loss, hipStream_t s) {
   k_xent_total<<<1, 1024, 0, s>>>(block_sum, n, a.reduction == 1, loss, a.count);
 }
-void factors(const XentArgs& a, const float* dloss, float* factor, unsigned* fmax, bool zeroed, hipStream_t s) {
-  const unsigned blocks = blocks_for(a.rows, 256 * 4, 256);
+void factors(const XentArgs& a, const float* dloss, float* factor, unsigned* fmax, bool zeroed, hipStream_t s,
+             const Magnitudes& mag) {
+  const unsigned blocks = blocks_for(mag.w && a.classes > a.rows ? a.classes : a.rows, 256 * 4, 256);
   if (blocks > 1 && !zeroed) k_zero_words<<<1, 64, 0, s>>>(fmax, 1);
-  k_xent_factor<<<blocks, 256, 0, s>>>(dloss, a.target, a.ignore, (int)a.classes, a.count, a.reduction, a.rows,
-                                       round_up(a.rows, 32), factor, fmax);
+  k_xent_factor<<<dim3(blocks, mag.w ? 2 : 1), 256, 0, s>>>(dloss, a.target, a.ignore, (int)a.classes, a.count, a.reduction,
+                                                            a.rows, round_up(a.rows, 32), factor, fmax, mag);
 }
 
 }  // namespace xent
@@ -484,15 +483,22 @@ size_t xent_backward(const XentArgs& a, const float* dloss, void* dh, void* dw, 
   if (few_backwards(a)) return few_backward(a, dloss, dh, dw, s);
   const bool go = a.ws != nullptr;
   Carver c(a.ws);
+  const bool scaled = a.dtype != kF16T;   // float16 inputs are operands as they are
   unsigned* words = c.take<unsigned>(3);
-  const Scalars sc{words, words + 1, words + 2};
+  const Scalars sc{scaled ? words : nullptr, scaled ? words + 1 : nullptr, words + 2};
   float* factor = c.take<float>(round_up(a.rows, 32));
+  float *max_h = scaled ? c.take<float>(a.rows) : nullptr, *max_w = scaled ? c.take<float>(a.classes) : nullptr;
+  const Logits lg(a, c, s, max_w, max_h);
   if (go) {
+    if (a.dtype == kBf16T) {
+      Pair<__bf16> pair{};
+      pair.m[0] = {(const __bf16*)a.w, a.ldw, a.classes, a.dim, nullptr, 0, nullptr, max_w, nullptr, nullptr, nullptr};
+      pair.m[1] = {(const __bf16*)a.h, a.ldh, a.rows, a.dim, nullptr, 0, nullptr, max_h, nullptr, nullptr, nullptr};
+      row_maxima(pair, 2, s);
+    }
     k_zero_words<<<1, 64, 0, s>>>(words, 3);
-    factors(a, dloss, factor, sc.gmax, true, s);
-    maxima(a, sc, s);
+    factors(a, dloss, factor, sc.gmax, true, s, {max_h, max_w, sc.h_largest, sc.w_largest});
   }
-  const Logits lg(a, c, s);
   size_t used = c.used;
   if (a.dtype == kF32T) backward_pieces<kSplit>(a, c, lg, sc, factor, dh, dw, s, used);
   else backward_pieces<kF16>(a, c, lg, sc, factor, dh, dw, s, used);

@@ -16,13 +16,13 @@ struct Out {
   int64_t ld;
   int dtype;
   const float* prev;        // null: none; [m][n] with n values a row
-  const unsigned* scale;    // the operand's scale, null: 1
+  const unsigned* largest;  // what the operand is scaled by (k_pack_t), null: it is not
   float alpha;
   const float* row;         // null: 1
   const unsigned* fmax;     // largest of the factors folded into an operand (k_pack_t), null: none
   int m, n;
   __device__ float factor() const {
-    return alpha * (scale ? inverse_scale(scale) : 1.f) * (fmax ? factor_unit(fmax) : 1.f);
+    return alpha * (largest ? power_of_two(-scale_exponent(largest, fmax)) : 1.f) * (fmax ? factor_unit(fmax) : 1.f);
   }
   // v is already times factor()
   __device__ float finish(int r, int c, float v) const {
@@ -45,9 +45,15 @@ struct Out {
 void join_parts(const float* part, int splits, const Out& o, hipStream_t s);
 // The loss over all rows and the number of labelled ones from n workgroups' sums of both.
 void total(const float2* block_sum, int n, const XentArgs& a, float* loss, hipStream_t s);
+// Rows' largest magnitudes, and where the largest exponents of h times its rows' factors and of w go; null: not wanted.
+struct Magnitudes {
+  const float *h, *w;
+  unsigned *h_largest, *w_largest;
+};
 // Rows' factors, zeros up to a multiple of 32 rows, and the largest of them
-// (zeroed: that is 0 already).
-void factors(const XentArgs& a, const float* dloss, float* factor, unsigned* fmax, bool zeroed, hipStream_t s);
+// (zeroed: that, and what else is joined, is 0 already).
+void factors(const XentArgs& a, const float* dloss, float* factor, unsigned* fmax, bool zeroed, hipStream_t s,
+             const Magnitudes& mag = {});
 
 // Rows' statistics, losses (loss: each, may be null) and sums (block_sum: one a row, may be
 // null) from `parts` parts [part][row] of few rows.

@@ -77,3 +77,61 @@ def test_a_large_class_leaves_the_others_logits(gpu, shape, dtype):
     lse = torch.logsumexp(h.double() @ w.double().t(), 1)
     ez = (h.shape[1] + 8) * U32 * (h.double().abs() @ w.double().abs().t()).max(dim=1).values   # sums in another order
     assert ((got - ref).abs() <= 2 * ez + 32 * U32 * (lse.abs() + ref + 1)).all()
+
+
+def _gradients(h, w, t, reduction="mean", up=None):
+    import torch
+    from mask_amd import ops
+    hl, wl = h.clone().requires_grad_(), w.clone().requires_grad_()
+    loss = ops.linear_cross_entropy(hl, wl, t, reduction=reduction)
+    return torch.autograd.grad(loss, (hl, wl), torch.ones_like(loss) if up is None else up)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", XENT_FORMS)
+def test_ignored_rows_change_no_gradient(gpu, shape, dtype):
+    """Equal bits: rows that do not count have no say in an operand's scale."""
+    import torch
+    h, w, t = _xent_case(*shape, dtype, seed=24, labelled=0.5)
+    off = (t == -100).nonzero().squeeze(1)
+    clean = _gradients(h, w, t)
+    assert clean[1].any() and not clean[0][off].any()
+    for value in _garbage(dtype):
+        _say("ignored rows, gradients", shape, dtype, value)
+        bad = h.clone()
+        bad[off[::2]] = value
+        bad[off[1], 3] = value
+        for a, b in zip(_gradients(bad, w, t), clean):
+            assert torch.equal(a, b), value
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shape", XENT_FORMS)
+def test_a_large_row_of_a_small_gradient(gpu, shape, dtype):
+    """A row of 1e6 whose upstream gradient is 1e-6 is a row like the others in the weight's gradient: 64 bits' within
+    the bound of its products (2^-21 of a 32-bit operand, 2^-11 of dz and of a row times its factor in 16 bits)."""
+    import torch
+    rows, _, classes = shape
+    h, w, t = _xent_case(*shape, dtype, seed=25, labelled=1.0)
+    h = h / 16          # logits that stay soft times 1e6 would be one-hot: that row's are made small by its weight below
+    w = w.clone()
+    w[:, 0] = 0
+    h[7] = 0
+    h[7, 0] = 1e6       # the only large feature meets weights of 0: the row's softmax is flat
+    up = torch.ones(rows, device="cuda")
+    up[7] = 1e-6
+    _say("large row of a small gradient", shape, dtype)
+    _, dw = _gradients(h, w, t, "none", up)
+    z = h.double() @ w.double().t()
+    dz = torch.softmax(z, 1)
+    dz.scatter_add_(1, t.unsqueeze(1), -torch.ones_like(t, dtype=torch.float64).unsqueeze(1))
+    dz *= up.double().unsqueeze(1)
+    want = dz.t() @ h.double()
+    size = dz.abs().t() @ h.double().abs()
+    ez = (2.0 ** -21 + (h.shape[1] + 8) * U32) * (h.double().abs() @ w.double().abs().t()).max()
+    half = 2.0 ** -24 if dtype == "float32" else 2.0 ** -8
+    keep = 2.0 ** -19 if dtype == "float32" else 2.0 ** -10 + 2.0 ** -20   # dz, a row times its factor, the other operand
+    # operands: 2^-40 of the largest entry (1e6 times 1e-6 and h's own) times the gradients' sum
+    edge = 2.0 ** -39 * (h[:7].double().abs().max() + 1) * dz.abs().sum(0).unsqueeze(1) + rows * 2.0 ** -38
+    bound = half * want.abs() + (keep + 2 * ez + (4 * rows ** 0.5 + 96) * U32) * size + edge
+    assert ((dw.double() - want).abs() <= bound).all(), ((dw.double() - want).abs() / bound).max().item()
