@@ -99,7 +99,7 @@ struct GradEpi : WaveEpi {
   Exponents ex;
   const float2* lse;             // row: largest logit, 1 / sum of exponentials
   const int64_t* target;
-  int64_t ignore;
+  const float* factor;           // a row of factor 0 has a dz of 0, whatever its logits
   char *dz, *dzt;                // [rows][classes of the piece], [classes of the piece][rows]
   int64_t ld, ldt;
   int rows, classes, first;      // first: the piece's first class
@@ -114,8 +114,8 @@ struct GradEpi : WaveEpi {
 #pragma unroll
     for (int j = 0; j < TJ; ++j) {
       const int t = col_of(w, j);
-      const int64_t tg = t < rows ? target[t] : ignore;
-      live[j] = tg != ignore;
+      live[j] = t < rows && factor[t] != 0.f;
+      const int64_t tg = live[j] ? target[t] : -1;
       st[j] = live[j] ? lse[t] : make_float2(0.f, 0.f);
       at[j] = tg >= first && tg < (int64_t)first + classes ? (int)(tg - first) : -1;
     }
@@ -400,7 +400,7 @@ void backward_pieces(const XentArgs& a, Carver& c, const Logits& lg, const Scala
       Operand wp = lg.w;
       wp.p = (const char*)wp.p + v0 * wp.ld;
       wp.rows = (int)n;
-      GradEpi<KIND> e{{}, {lg.ex.w ? lg.ex.w + v0 : nullptr, lg.ex.h}, (const float2*)a.lse, a.target, a.ignore, dz, dzt, ldz, ldzt,
+      GradEpi<KIND> e{{}, {lg.ex.w ? lg.ex.w + v0 : nullptr, lg.ex.h}, (const float2*)a.lse, a.target, factor, dz, dzt, ldz, ldzt,
                       (int)a.rows, (int)n, (int)v0};
       lg.run<KIND == kSplit, true>(cut, wp, a.dim, e, scratch, s);
     }

@@ -135,3 +135,24 @@ def test_a_large_row_of_a_small_gradient(gpu, shape, dtype):
     edge = 2.0 ** -39 * (h[:7].double().abs().max() + 1) * dz.abs().sum(0).unsqueeze(1) + rows * 2.0 ** -38
     bound = half * want.abs() + (keep + 2 * ez + (4 * rows ** 0.5 + 96) * U32) * size + edge
     assert ((dw.double() - want).abs() <= bound).all(), ((dw.double() - want).abs() / bound).max().item()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", XENT_FORMS)
+def test_rows_of_no_upstream_gradient_change_no_gradient(gpu, shape, dtype):
+    """A labelled row whose loss has an upstream gradient of 0 is a row of zeros in every gradient, whatever it holds
+    (its own loss is what it is)."""
+    import torch
+    h, w, t = _xent_case(*shape, dtype, seed=26, labelled=1.0)
+    off = torch.arange(0, shape[0], 3, device="cuda")
+    up = torch.linspace(0.5, 2.0, shape[0], device="cuda")
+    up[off] = 0
+    clean = _gradients(h, w, t, "none", up)
+    assert clean[1].any() and not clean[0][off].any()
+    for value in _garbage(dtype):
+        _say("no upstream gradient", shape, dtype, value)
+        bad = h.clone()
+        bad[off[::2]] = value
+        bad[off[1], 3] = value
+        for a, b in zip(_gradients(bad, w, t, "none", up), clean):
+            assert torch.equal(a, b), value
