@@ -64,6 +64,10 @@ def _like(t: Tensor) -> Tensor:
     return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
+def _dense(t: Optional[Tensor]) -> Optional[Tensor]:
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
 def _workspace(n: int, like: Tensor) -> Optional[Tensor]:
     return torch.empty(n, dtype=torch.uint8, device=like.device) if n > 1 else None
 
@@ -92,6 +96,20 @@ def _once(backward):
     wrapper that does so costs as much as a launch, so it is there only where the pass runs with gradients enabled."""
     checked = torch.autograd.function.once_differentiable(backward)
     return staticmethod(lambda ctx, g: checked(ctx, g) if torch.is_grad_enabled() else backward(ctx, g))
+
+
+# Hooks of saved tensors may give them back in another layout (save_on_cpu makes slices dense).  The
+# forward pass notes what its features are, and a backward pass that gets others describes them anew.  What is
+# looked at is kept short: on the engine's thread each of these costs a part of a launch.
+
+def _kind(t: Tensor):
+    return t.shape, t.stride(), t.dtype, t.is_cuda
+
+
+def _same_values(t: Tensor, kind) -> None:
+    """Raises where a saved tensor is not what it was but for its layout."""
+    if (t.shape, t.dtype, t.is_cuda) != (kind[0], kind[2], kind[3]):
+        raise RuntimeError(f"a saved tensor came back as {tuple(t.shape)}, {t.dtype} on {t.device}")
 
 
 # ---- group norm ---------------------------------------------------------------
@@ -149,9 +167,14 @@ def _norm_backward(ctx, dy):
     # the engine runs this on the device and the stream of the forward pass
     x, weight, bias, stats = ctx.saved_tensors
     groups, eps, act, xs, (desc, n) = ctx.args
-    if not dy.is_contiguous():
+    weight, bias, stats = _dense(weight), _dense(bias), _dense(stats)
+    same = _kind(x) == ctx.kind
+    if not same:
+        _same_values(x, ctx.kind)
+        x, *xs = _rows(x)
+    if not same or not dy.is_contiguous():
         dy, dsb, dld = _rows(dy)
-        desc, n = _norm_plan(x, xs, (dsb, dld), groups, weight if weight is not None else bias, eps, act, 1)
+        desc, n = _norm_plan(x, tuple(xs), (dsb, dld), groups, weight if weight is not None else bias, eps, act, 1)
     dx = _like(x)
     dw = _like(weight) if weight is not None and ctx.needs_input_grad[1] else None
     db = _like(bias) if bias is not None and ctx.needs_input_grad[2] else None
@@ -168,6 +191,7 @@ class _GroupNorm(torch.autograd.Function):
         x, sb, ld = _rows(x)
         y, stats = _norm_forward(x, sb, ld, weight, bias, groups, eps, act)
         ctx.save_for_backward(x, weight, bias, stats)
+        ctx.kind = _kind(x)
         # the description for a contiguous gradient, found here: the backward pass's thread is the slower one
         ctx.args = (groups, eps, act, (sb, ld), _norm_plan(x, (sb, ld), (y.stride(0), y.shape[-1]), groups,
                                                            weight if weight is not None else bias, eps, act, 1))
@@ -206,8 +230,7 @@ def group_norm(x: Tensor, num_groups: int, weight: Optional[Tensor] = None, bias
             raise ValueError(f"{name} must have one value a channel")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError("weight and bias must have one type")
-    weight = weight if weight is None else weight.contiguous()
-    bias = bias if bias is None else bias.contiguous()
+    weight, bias = _dense(weight), _dense(bias)
     act = _capi.ACTIVATIONS[activation]
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
@@ -245,11 +268,21 @@ def _xent_forward(h, weight, target, ignore, reduction):
     return loss, state
 
 
+def _xent_kinds(h, weight):
+    # operands that are not aligned are copied to the workspace
+    return _kind(h), _kind(weight), h.data_ptr() & 15, weight.data_ptr() & 15
+
+
 def _xent_backward(ctx, dloss):
     # the engine runs this on the device and the stream of the forward pass
     h, weight, target, state = ctx.saved_tensors
-    desc, n = ctx.plan
-    dloss = dloss.contiguous()
+    ignore, reduction, (desc, n) = ctx.args
+    target, state, dloss = _dense(target), _dense(state), _dense(dloss)
+    if _xent_kinds(h, weight) != ctx.kinds:
+        _same_values(h, ctx.kinds[0])
+        _same_values(weight, ctx.kinds[1])
+        h, weight = _matrix(h), _matrix(weight)
+        desc, n = _xent_plan(h, weight, ignore, reduction, 1)
     dh = _like(h) if ctx.needs_input_grad[0] else None
     dw = _like(weight) if ctx.needs_input_grad[1] else None
     ws = _workspace(n, h)
@@ -265,7 +298,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
         hm, wm = _matrix(h), _matrix(weight)
         loss, state = _xent_forward(hm, wm, target, ignore, reduction)
         ctx.save_for_backward(hm, wm, target, state)
-        ctx.plan = _xent_plan(hm, wm, ignore, reduction, 1)
+        ctx.kinds = _xent_kinds(hm, wm)
+        ctx.args = (ignore, reduction, _xent_plan(hm, wm, ignore, reduction, 1))
         return loss
 
     backward = _once(_xent_backward)
@@ -296,7 +330,7 @@ def linear_cross_entropy(h: Tensor, weight: Tensor, target: Tensor, ignore_index
         raise RuntimeError(f"target is on {target.device}, expected {h.device}")
     if reduction not in _capi.REDUCTIONS:
         raise ValueError(f"unknown reduction {reduction!r} ({', '.join(_capi.REDUCTIONS)})")
-    target = target.contiguous()
+    target = _dense(target)
     code = _capi.REDUCTIONS[reduction]
     if torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad):
         return _LinearCrossEntropy.apply(h, weight, target, int(ignore_index), code)

@@ -4,7 +4,7 @@ from __future__ import annotations
 
 import pytest
 
-from tests.test_gpu_ops import DTYPES, U32, _say, _xent_case
+from tests.test_gpu_ops import DTYPES, U32, _norm_case, _say, _xent_case
 
 pytestmark = pytest.mark.gpu
 
@@ -156,3 +156,63 @@ def test_rows_of_no_upstream_gradient_change_no_gradient(gpu, shape, dtype):
         bad[off[1], 3] = value
         for a, b in zip(_gradients(bad, w, t, "none", up), clean):
             assert torch.equal(a, b), value
+
+
+# ---- saved tensors that come back in another layout ------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_saved_tensors_may_come_back_in_another_layout(gpu, dtype):
+    """save_on_cpu makes a slice dense, and another hook gives back a slice of something wider or something that starts
+    elsewhere: the gradients keep their bits.  A tensor of another type or shape is refused."""
+    import torch
+    from mask_amd import ops
+
+    def wider(t):
+        if t.dim() < 2 or not t.is_floating_point():
+            return t.clone()
+        out = torch.zeros((*t.shape[:-1], t.shape[-1] + 24), dtype=t.dtype, device=t.device)[..., 8:8 + t.shape[-1]]
+        return out.copy_(t)
+
+    def shifted(t):
+        return torch.zeros(t.numel() + 1, dtype=t.dtype, device=t.device)[1:].copy_(t.reshape(-1)).view(t.shape)
+
+    hooks = {"plain": None, "save_on_cpu": torch.autograd.graph.save_on_cpu(),
+             "wider": torch.autograd.graph.saved_tensors_hooks(lambda t: t, wider),
+             "dense": torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.contiguous()),
+             # matrices only: statistics are aligned by contract, and group norm's loads, so the order of its sums, go by alignment
+             "shifted": torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: shifted(t) if t.dim() == 2 else t.clone())}
+    calls = []
+    for shape in ((130, 64, 300), (300, 64, 300), (90, 64, 70), (90, 64, 300)):
+        h, w, t = _xent_case(*shape, dtype, seed=31)
+        hw = torch.zeros(shape[0], 3 * shape[1], dtype=h.dtype, device="cuda")
+        ww = torch.zeros(shape[2], 2 * shape[1], dtype=h.dtype, device="cuda")
+        hc, wc = hw[:, 64:128].copy_(h), ww[:, 64:].copy_(w)
+        calls.append((shape, (hc, wc), lambda a, b, t=t: ops.linear_cross_entropy(a, b, t)))
+    for shape, groups in (((3, 40, 32), 4), ((2, 3000, 24), 6), ((500, 1, 64), 8), ((1, 9000, 16), 2)):
+        x, w, b, dy = _norm_case(shape, groups, "silu", dtype, seed=32)
+        wide = torch.zeros(shape[0], 2 * shape[1], shape[2] + 8, dtype=x.dtype, device="cuda")
+        xc = wide[:, shape[1]:, 8:].copy_(x)
+        calls.append((shape, (xc, w, b), lambda a, g, o, groups=groups, dy=dy:
+                      (ops.group_norm(a, groups, g, o, activation="silu") * dy).sum()))
+    for shape, ins, fn in calls:
+        want = None
+        for name, hook in hooks.items():
+            _say("saved tensors", shape, dtype, name)
+            leaves = [v.detach().requires_grad_() for v in ins]
+            if hook is None:
+                out = fn(*leaves)
+            else:
+                with hook:
+                    out = fn(*leaves)
+            got = torch.autograd.grad(out, leaves)
+            want = got if want is None else want
+            for a, b in zip(got, want):
+                assert torch.equal(a, b), name
+    for bad in (lambda t: t.double() if t.is_floating_point() else t, lambda t: t[:-1]):
+        for shape, ins, fn in (calls[0], calls[-1]):
+            leaves = [v.detach().requires_grad_() for v in ins]
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, bad):
+                out = fn(*leaves) if len(ins) == 2 else ops.group_norm(leaves[0], 2, leaves[1], leaves[2])
+            out = out.sum()
+            with pytest.raises(RuntimeError, match="came back as"):
+                torch.autograd.grad(out, leaves)
