@@ -884,46 +884,68 @@ __global__ __launch_bounds__(256) void k_norm_bwd_sums(Shape sh, Chunks ch, cons
   }
 }
 
-// The first group_blocks workgroups of a row of the grid: sums of du w and du w
-// xhat of a group of a sample.  The others: of du xhat and du of 16 channels.
-// blockIdx.y: the share of the parts; one share is the end already.
+// How a backward pass's parts are joined: one after the other in the grid, `groups` workgroups a share of the
+// groups' sums, then `params` a share of the parameters'.  Each has as many shares as its own parts ask for:
+// many short samples have few parts a group, and many of a parameter (8192 x 100 x 320 in 32 groups).
+struct BackwardJoin {
+  int groups, group_shares;
+  int params, param_shares;
+};
+
+// Sums of du w and du w xhat of a group of a sample; of du xhat and du of 16 channels.
+// One share is the end already.  Of up to 64 parts a wave joins a group, of more a workgroup.
 __global__ __launch_bounds__(256) void k_norm_bwd_join(Shape sh, int chunks, const float2* __restrict__ part, int64_t parts,
-                                                       int group_blocks, float2* __restrict__ group_shares,
+                                                       BackwardJoin jn, float2* __restrict__ group_shares,
                                                        float2* __restrict__ means, float2* __restrict__ param_shares,
                                                        void* __restrict__ dweight, void* __restrict__ dbias) {
   __shared__ float2 red[256];
+  const int group_blocks = jn.groups * jn.group_shares;
   if ((int)blockIdx.x < group_blocks) {
-    for (int64_t ng = blockIdx.x; ng < sh.batch * sh.groups; ng += group_blocks) {
+    const int all = chunks * sh.per_group;
+    const float inv = 1.f / ((float)sh.length * sh.per_group);
+    auto sum = [&](int64_t ng, int first, int step) {
       const int64_t n = ng / sh.groups;
       const int g = (int)(ng - n * sh.groups);
       float2 a = make_float2(0.f, 0.f);
-      const int all = chunks * sh.per_group;
-      for (int i = blockIdx.y * 256 + threadIdx.x; i < all; i += gridDim.y * 256) {
+      for (int i = first; i < all; i += step) {
         const int k = i / sh.per_group, c = g * sh.per_group + i - k * sh.per_group;
         const float2 o = part[(n * chunks + k) * sh.channels + c];
         const float w = param(sh.weight, sh.param_dtype, c, 1.f);
         a.x = fmaf(w, o.y, a.x), a.y = fmaf(w, o.x, a.y);
       }
-      red[threadIdx.x] = a;
+      return a;
+    };
+    if (all <= 64) {
+      for (int64_t ng = blockIdx.x * 4 + (threadIdx.x >> 6); ng < sh.batch * sh.groups; ng += jn.groups * 4) {
+        float2 a = sum(ng, threadIdx.x & 63, 64);
+#pragma unroll
+        for (int d = 32; d; d >>= 1) a.x += __shfl_xor(a.x, d), a.y += __shfl_xor(a.y, d);
+        if ((threadIdx.x & 63) == 0) means[ng] = make_float2(a.x * inv, a.y * inv);
+      }
+      return;
+    }
+    const int share = (int)blockIdx.x / jn.groups;
+    for (int64_t ng = (int)blockIdx.x - share * jn.groups; ng < sh.batch * sh.groups; ng += jn.groups) {
+      red[threadIdx.x] = sum(ng, share * 256 + threadIdx.x, jn.group_shares * 256);
       __syncthreads();
       for (int d = 128; d; d >>= 1) {
         if ((int)threadIdx.x < d) red[threadIdx.x].x += red[threadIdx.x + d].x, red[threadIdx.x].y += red[threadIdx.x + d].y;
         __syncthreads();
       }
       if (threadIdx.x == 0) {
-        const float inv = 1.f / ((float)sh.length * sh.per_group);
-        if (gridDim.y == 1) means[ng] = make_float2(red[0].x * inv, red[0].y * inv);
-        else group_shares[ng * gridDim.y + blockIdx.y] = red[0];
+        if (jn.group_shares == 1) means[ng] = make_float2(red[0].x * inv, red[0].y * inv);
+        else group_shares[ng * jn.group_shares + share] = red[0];
       }
       __syncthreads();
     }
     return;
   }
-  const int c = ((int)blockIdx.x - group_blocks) * 16 + (threadIdx.x & 15), sub = threadIdx.x >> 4;
+  const int id = (int)blockIdx.x - group_blocks, share = id / jn.params;
+  const int c = (id - share * jn.params) * 16 + (threadIdx.x & 15), sub = threadIdx.x >> 4;
   float2 a = make_float2(0.f, 0.f);
   if (c < sh.channels) {
 #pragma unroll 4
-    for (int64_t p = blockIdx.y * 16 + sub; p < parts; p += gridDim.y * 16) {
+    for (int64_t p = share * 16 + sub; p < parts; p += jn.param_shares * 16) {
       const float2 o = part[p * sh.channels + c];
       a.x += o.x, a.y += o.y;
     }
@@ -939,14 +961,14 @@ __global__ __launch_bounds__(256) void k_norm_bwd_join(Shape sh, int chunks, con
     __syncthreads();
   }
   if (sub || c >= sh.channels) return;
-  if (gridDim.y == 1) {
+  if (jn.param_shares == 1) {
     if (dweight) put_param(dweight, sh.param_dtype, c, a.x);
     if (dbias) put_param(dbias, sh.param_dtype, c, a.y);
   } else {
-    param_shares[(int64_t)blockIdx.y * sh.channels + c] = a;
+    param_shares[(int64_t)share * sh.channels + c] = a;
   }
 }
-// The shares' sums: means of the groups, gradients of the parameters.
+// The shares' sums: means of n_groups groups, gradients of the parameters (n_param 0: there is nothing to do for either).
 __global__ __launch_bounds__(256) void k_norm_bwd_end(Shape sh, int64_t n_groups, int n_shares,
                                                       const float2* __restrict__ group_shares, float2* __restrict__ means,
                                                       int n_param, const float2* __restrict__ param_shares,
@@ -1150,10 +1172,11 @@ int shares_of(int64_t parts, int64_t share) {
   const int64_t n = (parts + share - 1) / share;
   return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }
-// of a backward pass: its groups' parts and its parameters' are shared out alike
-int backward_shares(const NormArgs& a, int64_t count) {
-  const int g = shares_of(count * (a.channels / a.groups), kJoinShare), p = shares_of(a.batch * count, 256);
-  return g > p ? g : p;
+// of a backward pass in `count` chunks a sample
+BackwardJoin backward_join(const NormArgs& a, int64_t count, bool params) {
+  const int64_t parts = count * (a.channels / a.groups), all = a.batch * a.groups, blocks = parts <= 64 ? (all + 3) / 4 : all;
+  return {(int)(blocks < 65536 ? blocks : 65536), shares_of(parts, kJoinShare), params ? (int)((a.channels + 15) / 16) : 0,
+          shares_of(a.batch * count, 256)};
 }
 unsigned grid_z(int64_t batch) { return (unsigned)(batch < 65535 ? batch : 65535); }
 
@@ -1181,14 +1204,14 @@ size_t norm_workspace(const NormArgs& a, bool backward) {
       }
     } else {
       const int64_t count = chunks_of(a, v, grid_z(a.batch)).count;
-      const int shares = backward ? backward_shares(a, count) : shares_of(count * (a.channels / a.groups), kJoinShare);
       c.take<float2>(a.batch * count * a.channels);
       if (backward) {
-        c.take<float2>(a.batch * a.groups * shares);
+        const BackwardJoin jn = backward_join(a, count, true);
+        c.take<float2>(a.batch * a.groups * jn.group_shares);
         c.take<float2>(a.batch * a.groups);
-        c.take<float2>((size_t)shares * a.channels);
+        c.take<float2>((size_t)jn.param_shares * a.channels);
       } else {
-        c.take<Share>(a.batch * a.groups * shares);
+        c.take<Share>(a.batch * a.groups * shares_of(count * (a.channels / a.groups), kJoinShare));
       }
     }
     if (c.used > most) most = c.used;
@@ -1238,7 +1261,6 @@ void norm_backward(const NormArgs& a, const void* dy, int64_t lddy, int64_t batc
   const SmallPlan sp = small_plan(a, v);
   const Shape sh = shape_of(a, lddy, batch_dy);
   const bool params = dweight || dbias;
-  const unsigned param_blocks = params ? (unsigned)((a.channels + 15) / 16) : 0;
   Carver c(a.ws);
   if (sp.ok) {
     float2* part = c.take<float2>((size_t)sp.blocks * a.channels);
@@ -1255,8 +1277,9 @@ void norm_backward(const NormArgs& a, const void* dy, int64_t lddy, int64_t batc
     });
     if (params) {
       const int n = shares_of(sp.blocks, 256);
+      const BackwardJoin jn{0, 0, (int)((a.channels + 15) / 16), n};
       float2* shares = c.take<float2>((size_t)n * a.channels);
-      k_norm_bwd_join<<<dim3(param_blocks, n), 256, 0, s>>>(sh, 0, part, sp.blocks, 0, nullptr, nullptr, shares, dweight, dbias);
+      k_norm_bwd_join<<<(unsigned)(jn.params * n), 256, 0, s>>>(sh, 0, part, sp.blocks, jn, nullptr, nullptr, shares, dweight, dbias);
       if (n > 1)
         k_norm_bwd_end<<<(unsigned)((a.channels + 255) / 256), 256, 0, s>>>(sh, 0, 0, nullptr, nullptr, n, shares, dweight, dbias);
     }
@@ -1265,22 +1288,24 @@ void norm_backward(const NormArgs& a, const void* dy, int64_t lddy, int64_t batc
   const unsigned z = grid_z(a.batch);
   const Chunks ch = chunks_of(a, v, z);
   float2* part = c.take<float2>(a.batch * ch.count * a.channels);
-  const int n_shares = backward_shares(a, ch.count);
-  float2* group_shares = c.take<float2>(a.batch * a.groups * n_shares);
+  const BackwardJoin jn = backward_join(a, ch.count, params);
+  float2* group_shares = c.take<float2>(a.batch * a.groups * jn.group_shares);
   float2* means = c.take<float2>(a.batch * a.groups);
-  float2* param_shares = c.take<float2>((size_t)n_shares * a.channels);
+  float2* param_shares = c.take<float2>((size_t)jn.param_shares * a.channels);
   by_type(a.dtype, [&](auto* t) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
     by_vector<T>(v, [&](auto vc) {
       constexpr int V = decltype(vc)::value;
       const dim3 grid(ch.count, ch.tiles, z);
       k_norm_bwd_sums<T, V><<<grid, 256, 0, s>>>(sh, ch, (const T*)a.x, (const T*)dy, (const float4*)a.stats, part);
-      const int64_t ng = a.batch * a.groups;
-      const unsigned gb = (unsigned)(ng < 65536 ? ng : 65536);
-      k_norm_bwd_join<<<dim3(gb + param_blocks, n_shares), 256, 0, s>>>(sh, ch.count, part, a.batch * ch.count, (int)gb,
-                                                                         group_shares, means, param_shares, dweight, dbias);
-      if (n_shares > 1) k_norm_bwd_end<<<(unsigned)((ng + a.channels + 255) / 256), 256, 0, s>>>(sh, ng, n_shares, group_shares, means,
-                                                                              params ? n_shares : 0, param_shares, dweight, dbias);
+      k_norm_bwd_join<<<(unsigned)(jn.groups * jn.group_shares + jn.params * jn.param_shares), 256, 0, s>>>(
+          sh, ch.count, part, a.batch * ch.count, jn, group_shares, means, param_shares, dweight, dbias);
+      // what is not in shares is done
+      const int64_t ng = jn.group_shares > 1 ? a.batch * a.groups : 0;
+      const int np = params && jn.param_shares > 1 ? jn.param_shares : 0;
+      if (ng || np)
+        k_norm_bwd_end<<<(unsigned)((ng + (np ? a.channels : 0) + 255) / 256), 256, 0, s>>>(
+            sh, ng, jn.group_shares, group_shares, means, np, param_shares, dweight, dbias);
       k_norm_bwd_apply<T, V><<<grid, 256, 0, s>>>(sh, ch, (const T*)a.x, (const T*)dy, (T*)dx, (const float4*)a.stats, means);
     });
   });

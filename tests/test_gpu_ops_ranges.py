@@ -4,7 +4,7 @@ from __future__ import annotations
 
 import pytest
 
-from tests.test_gpu_ops import DTYPES, U32, _norm_case, _say, _xent_case
+from tests.test_gpu_ops import DTYPES, U32, _check_norm, _norm_case, _say, _xent_case
 
 pytestmark = pytest.mark.gpu
 
@@ -216,3 +216,14 @@ def test_saved_tensors_may_come_back_in_another_layout(gpu, dtype):
             out = out.sum()
             with pytest.raises(RuntimeError, match="came back as"):
                 torch.autograd.grad(out, leaves)
+
+
+# ---- group norm of many samples --------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shape, groups", [((2048, 50, 320), 32), ((2048, 50, 320), 2), ((600, 130, 256), 256), ((70, 700, 200), 1)])
+def test_group_norm_of_many_split_samples(gpu, shape, groups, dtype):
+    """Samples of a chunk or a few each: groups of few parts, parameters of many."""
+    x, w, b, dy = _norm_case(shape, groups, "silu", dtype, seed=41)
+    _say("many split samples", shape, groups, dtype)
+    _check_norm(x, groups, w, b, dy, "silu", what=f"{shape} {groups} {dtype}")

@@ -199,3 +199,13 @@ def test_host_tensors_are_refused():
         ops.orthogonalize(x)
     with pytest.raises(TypeError, match="torch tensor"):
         ops.orthogonalize([[1.0]])
+
+
+def test_group_norm_workspace_of_many_short_samples():
+    """Split samples of one chunk each have few parts a group, however many of them the parameters' gradients are
+    joined from: the parts, two means a group and at most 64 shares of the parameters."""
+    batch, length, channels, groups = 8192, 100, 320, 32
+    d = _norm(batch=batch, length=length, channels=channels, groups=groups, batch_x=length * channels, ld_x=channels,
+              batch_dy=length * channels, ld_dy=channels)
+    rc, n = _norm_size(d, 1)
+    assert rc == 0 and n <= 8 * (batch * channels + 2 * batch * groups + 64 * channels) + 4 * 256
