@@ -353,12 +353,12 @@ __device__ __forceinline__ void put_params(const Shape& sh, bool on, int row, in
 __device__ __forceinline__ void join_params(const Shape& sh, int rows, const float2* lds, float2* __restrict__ part) {
   __syncthreads();
   for (int c = threadIdx.x; c < sh.channels; c += blockDim.x) {
-    float2 a = make_float2(0.f, 0.f);
+    double2 a = make_double2(0., 0.);
     for (int r = 0; r < rows; ++r) {
       const float2 o = lds[r * sh.channels + c];
       a.x += o.x, a.y += o.y;
     }
-    part[(int64_t)blockIdx.x * sh.channels + c] = a;
+    part[(int64_t)blockIdx.x * sh.channels + c] = make_float2((float)a.x, (float)a.y);
   }
 }
 
@@ -873,12 +873,12 @@ __global__ __launch_bounds__(256) void k_norm_bwd_sums(Shape sh, Chunks ch, cons
     for (int k = threadIdx.x; k < width; k += 256) {
       const int c = blockIdx.y * width + k;
       if (c >= sh.channels) break;
-      float2 a = make_float2(0.f, 0.f);
+      double2 a = make_double2(0., 0.);
       for (int t = 0; t < ch.row_threads; ++t) {
         const float2 o = red[t * width + k];
         a.x += o.x, a.y += o.y;
       }
-      part[(n * ch.count + blockIdx.x) * sh.channels + c] = a;
+      part[(n * ch.count + blockIdx.x) * sh.channels + c] = make_float2((float)a.x, (float)a.y);
     }
     __syncthreads();
   }
@@ -895,32 +895,33 @@ struct BackwardJoin {
 // Sums of du w and du w xhat of a group of a sample; of du xhat and du of 16 channels.
 // One share is the end already.  Of up to 64 parts a wave joins a group, of more a workgroup.
 __global__ __launch_bounds__(256) void k_norm_bwd_join(Shape sh, int chunks, const float2* __restrict__ part, int64_t parts,
-                                                       BackwardJoin jn, float2* __restrict__ group_shares,
-                                                       float2* __restrict__ means, float2* __restrict__ param_shares,
+                                                       BackwardJoin jn, double2* __restrict__ group_shares,
+                                                       float2* __restrict__ means, double2* __restrict__ param_shares,
                                                        void* __restrict__ dweight, void* __restrict__ dbias) {
-  __shared__ float2 red[256];
+  __shared__ double2 red[256];
   const int group_blocks = jn.groups * jn.group_shares;
   if ((int)blockIdx.x < group_blocks) {
     const int all = chunks * sh.per_group;
-    const float inv = 1.f / ((float)sh.length * sh.per_group);
+    const double inv = 1. / ((double)sh.length * sh.per_group);
+    auto mean = [&](double2 a) { return make_float2((float)(a.x * inv), (float)(a.y * inv)); };
     auto sum = [&](int64_t ng, int first, int step) {
       const int64_t n = ng / sh.groups;
       const int g = (int)(ng - n * sh.groups);
-      float2 a = make_float2(0.f, 0.f);
+      double2 a = make_double2(0., 0.);
       for (int i = first; i < all; i += step) {
         const int k = i / sh.per_group, c = g * sh.per_group + i - k * sh.per_group;
         const float2 o = part[(n * chunks + k) * sh.channels + c];
-        const float w = param(sh.weight, sh.param_dtype, c, 1.f);
-        a.x = fmaf(w, o.y, a.x), a.y = fmaf(w, o.x, a.y);
+        const double w = param(sh.weight, sh.param_dtype, c, 1.f);
+        a.x = fma(w, (double)o.y, a.x), a.y = fma(w, (double)o.x, a.y);
       }
       return a;
     };
     if (all <= 64) {
       for (int64_t ng = blockIdx.x * 4 + (threadIdx.x >> 6); ng < sh.batch * sh.groups; ng += jn.groups * 4) {
-        float2 a = sum(ng, threadIdx.x & 63, 64);
+        double2 a = sum(ng, threadIdx.x & 63, 64);
 #pragma unroll
         for (int d = 32; d; d >>= 1) a.x += __shfl_xor(a.x, d), a.y += __shfl_xor(a.y, d);
-        if ((threadIdx.x & 63) == 0) means[ng] = make_float2(a.x * inv, a.y * inv);
+        if ((threadIdx.x & 63) == 0) means[ng] = mean(a);
       }
       return;
     }
@@ -933,7 +934,7 @@ __global__ __launch_bounds__(256) void k_norm_bwd_join(Shape sh, int chunks, con
         __syncthreads();
       }
       if (threadIdx.x == 0) {
-        if (jn.group_shares == 1) means[ng] = make_float2(red[0].x * inv, red[0].y * inv);
+        if (jn.group_shares == 1) means[ng] = mean(red[0]);
         else group_shares[ng * jn.group_shares + share] = red[0];
       }
       __syncthreads();
@@ -942,7 +943,7 @@ __global__ __launch_bounds__(256) void k_norm_bwd_join(Shape sh, int chunks, con
   }
   const int id = (int)blockIdx.x - group_blocks, share = id / jn.params;
   const int c = (id - share * jn.params) * 16 + (threadIdx.x & 15), sub = threadIdx.x >> 4;
-  float2 a = make_float2(0.f, 0.f);
+  double2 a = make_double2(0., 0.);
   if (c < sh.channels) {
 #pragma unroll 4
     for (int64_t p = share * 16 + sub; p < parts; p += jn.param_shares * 16) {
@@ -954,7 +955,7 @@ __global__ __launch_bounds__(256) void k_norm_bwd_join(Shape sh, int chunks, con
   __syncthreads();
   for (int d = 8; d; d >>= 1) {
     if (sub < d) {
-      const float2 o = red[threadIdx.x + 16 * d];
+      const double2 o = red[threadIdx.x + 16 * d];
       a.x += o.x, a.y += o.y;
       red[threadIdx.x] = a;
     }
@@ -962,34 +963,34 @@ __global__ __launch_bounds__(256) void k_norm_bwd_join(Shape sh, int chunks, con
   }
   if (sub || c >= sh.channels) return;
   if (jn.param_shares == 1) {
-    if (dweight) put_param(dweight, sh.param_dtype, c, a.x);
-    if (dbias) put_param(dbias, sh.param_dtype, c, a.y);
+    if (dweight) put_param(dweight, sh.param_dtype, c, (float)a.x);
+    if (dbias) put_param(dbias, sh.param_dtype, c, (float)a.y);
   } else {
     param_shares[(int64_t)share * sh.channels + c] = a;
   }
 }
 // The shares' sums: means of n_groups groups, gradients of the parameters (n_param 0: there is nothing to do for either).
 __global__ __launch_bounds__(256) void k_norm_bwd_end(Shape sh, int64_t n_groups, int n_shares,
-                                                      const float2* __restrict__ group_shares, float2* __restrict__ means,
-                                                      int n_param, const float2* __restrict__ param_shares,
+                                                      const double2* __restrict__ group_shares, float2* __restrict__ means,
+                                                      int n_param, const double2* __restrict__ param_shares,
                                                       void* __restrict__ dweight, void* __restrict__ dbias) {
   int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  float2 a = make_float2(0.f, 0.f);
+  double2 a = make_double2(0., 0.);
   if (i < n_groups) {
     for (int k = 0; k < n_shares; ++k) {
-      const float2 o = group_shares[i * n_shares + k];
+      const double2 o = group_shares[i * n_shares + k];
       a.x += o.x, a.y += o.y;
     }
-    const float inv = 1.f / ((float)sh.length * sh.per_group);
-    means[i] = make_float2(a.x * inv, a.y * inv);
+    const double inv = 1. / ((double)sh.length * sh.per_group);
+    means[i] = make_float2((float)(a.x * inv), (float)(a.y * inv));
   } else if (i - n_groups < sh.channels && n_param) {
     i -= n_groups;
     for (int k = 0; k < n_param; ++k) {
-      const float2 o = param_shares[(int64_t)k * sh.channels + i];
+      const double2 o = param_shares[(int64_t)k * sh.channels + i];
       a.x += o.x, a.y += o.y;
     }
-    if (dweight) put_param(dweight, sh.param_dtype, i, a.x);
-    if (dbias) put_param(dbias, sh.param_dtype, i, a.y);
+    if (dweight) put_param(dweight, sh.param_dtype, i, (float)a.x);
+    if (dbias) put_param(dbias, sh.param_dtype, i, (float)a.y);
   }
 }
 
@@ -1200,16 +1201,16 @@ size_t norm_workspace(const NormArgs& a, bool backward) {
     if (sp.ok) {
       if (backward) {
         c.take<float2>((size_t)sp.blocks * a.channels);
-        c.take<float2>((size_t)shares_of(sp.blocks, 256) * a.channels);
+        c.take<double2>((size_t)shares_of(sp.blocks, 256) * a.channels);
       }
     } else {
       const int64_t count = chunks_of(a, v, grid_z(a.batch)).count;
       c.take<float2>(a.batch * count * a.channels);
       if (backward) {
         const BackwardJoin jn = backward_join(a, count, true);
-        c.take<float2>(a.batch * a.groups * jn.group_shares);
+        c.take<double2>(jn.group_shares > 1 ? a.batch * a.groups * jn.group_shares : 0);
         c.take<float2>(a.batch * a.groups);
-        c.take<float2>((size_t)jn.param_shares * a.channels);
+        c.take<double2>((size_t)jn.param_shares * a.channels);
       } else {
         c.take<Share>(a.batch * a.groups * shares_of(count * (a.channels / a.groups), kJoinShare));
       }
@@ -1278,7 +1279,7 @@ void norm_backward(const NormArgs& a, const void* dy, int64_t lddy, int64_t batc
     if (params) {
       const int n = shares_of(sp.blocks, 256);
       const BackwardJoin jn{0, 0, (int)((a.channels + 15) / 16), n};
-      float2* shares = c.take<float2>((size_t)n * a.channels);
+      double2* shares = c.take<double2>((size_t)n * a.channels);
       k_norm_bwd_join<<<(unsigned)(jn.params * n), 256, 0, s>>>(sh, 0, part, sp.blocks, jn, nullptr, nullptr, shares, dweight, dbias);
       if (n > 1)
         k_norm_bwd_end<<<(unsigned)((a.channels + 255) / 256), 256, 0, s>>>(sh, 0, 0, nullptr, nullptr, n, shares, dweight, dbias);
@@ -1289,9 +1290,9 @@ void norm_backward(const NormArgs& a, const void* dy, int64_t lddy, int64_t batc
   const Chunks ch = chunks_of(a, v, z);
   float2* part = c.take<float2>(a.batch * ch.count * a.channels);
   const BackwardJoin jn = backward_join(a, ch.count, params);
-  float2* group_shares = c.take<float2>(a.batch * a.groups * jn.group_shares);
+  double2* group_shares = c.take<double2>(jn.group_shares > 1 ? a.batch * a.groups * jn.group_shares : 0);
   float2* means = c.take<float2>(a.batch * a.groups);
-  float2* param_shares = c.take<float2>((size_t)jn.param_shares * a.channels);
+  double2* param_shares = c.take<double2>((size_t)jn.param_shares * a.channels);
   by_type(a.dtype, [&](auto* t) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
     by_vector<T>(v, [&](auto vc) {

@@ -227,3 +227,35 @@ def test_group_norm_of_many_split_samples(gpu, shape, groups, dtype):
     x, w, b, dy = _norm_case(shape, groups, "silu", dtype, seed=41)
     _say("many split samples", shape, groups, dtype)
     _check_norm(x, groups, w, b, dy, "silu", what=f"{shape} {groups} {dtype}")
+
+
+@pytest.mark.parametrize("shape, groups, rows", [((1, 1000003, 8), 8, 4), ((3000000, 1, 4), 2, 23), ((65536, 30, 8), 2, 8)])
+def test_group_norm_parameter_gradients_of_many_rows(gpu, shape, groups, rows):
+    """Sums over millions of rows for few channels, a shape for each form: a thread adds `rows` values in 32 bits, the
+    threads' sums are joined in 64, what a workgroup has is rounded once and so is the result.  In units of 2^-24 of
+    the root of the sum of squares, roundings of random sign then come to sqrt((rows / 2 + 2) / 3); the root mean
+    square over channels and seeds stays below 1.5 times that (a chain of 128 threads in 32 bits: 4.6 and more).  Of the
+    weight's gradient as well, whose terms have two roundings more."""
+    import torch
+    from mask_amd import ops
+    units = {"dweight": [], "dbias": []}
+    for seed in range(4):
+        _say("parameter gradients", shape, seed)
+        gen = torch.Generator(device="cuda")
+        gen.manual_seed(seed)
+        x = torch.randn(shape, generator=gen, device="cuda")
+        dy = torch.randn(shape, generator=gen, device="cuda")
+        w = torch.ones(shape[-1], device="cuda", requires_grad=True)
+        b = torch.zeros(shape[-1], device="cuda", requires_grad=True)
+        dw, db = torch.autograd.grad(ops.group_norm(x, groups, w, b, eps=0.1), (w, b), dy)
+        d = dy.double()
+        units["dbias"].append((db.double() - d.sum(dim=(0, 1))) / (U32 * (d * d).sum(dim=(0, 1)).sqrt()))
+        if shape[1] > 1:
+            v = x.double().reshape(shape[0], shape[1], groups, -1)
+            var, mean = torch.var_mean(v, dim=(1, 3), unbiased=False, keepdim=True)
+            d = d * ((v - mean) / (var + 0.1).sqrt()).reshape(shape)
+            units["dweight"].append((dw.double() - d.sum(dim=(0, 1))) / (U32 * (d * d).sum(dim=(0, 1)).sqrt()))
+    for (what, u), more in zip(units.items(), (2, 0)):
+        if u:
+            rms = torch.stack(u).square().mean().sqrt().item()
+            assert rms <= 1.5 * ((rows / 2 + 2 + more) / 3) ** 0.5, (what, rms)
