@@ -4,7 +4,7 @@ from __future__ import annotations
 
 import pytest
 
-from tests.test_gpu_ops import DTYPES, U32, _check_norm, _norm_case, _say, _xent_case
+from tests.test_gpu_ops import DTYPES, U32, _check_norm, _norm64, _norm_case, _say, _within, _xent_case
 
 pytestmark = pytest.mark.gpu
 
@@ -259,3 +259,39 @@ def test_group_norm_parameter_gradients_of_many_rows(gpu, shape, groups, rows):
         if u:
             rms = torch.stack(u).square().mean().sqrt().item()
             assert rms <= 1.5 * ((rows / 2 + 2 + more) / 3) ** 0.5, (what, rms)
+
+
+@pytest.mark.parametrize("shape, groups", [((70, 1, 4096), 512), ((3, 1, 768), 256), ((5, 1, 500), 1), ((1, 1, 8192), 8)])
+def test_group_norm_relu_knows_its_side(gpu, shape, groups):
+    """Single float32 rows: biases that take u to the rounding of a 32-bit number away from 0, about 1e-8, on either
+    side.  y is positive where 64 bits say so, and so the slope: no gradient is masked.  What 64 bits themselves leave
+    open (1e-12) is left out."""
+    import torch
+    from mask_amd import ops
+    n, _, c = shape
+    gen = torch.Generator().manual_seed(51)
+    x = (torch.randn(1, 1, c, generator=gen) + 3.0).cuda().expand(shape).contiguous()
+    w = (1 + 0.3 * torch.randn(c, generator=gen)).cuda()
+    dy = torch.randn(shape, generator=gen).cuda()
+    _, _, hat, _, rstd = _norm64(x.double(), groups, w.double(), torch.zeros_like(w).double(), 1e-5, "none")
+    b = (-hat[0, 0] * w.double()).float()
+    _, u, _, _, _ = _norm64(x.double(), groups, w.double(), b.double(), 1e-5, "relu")
+    open_ = u.abs() < 1e-12
+    assert (u.abs() < 1e-6).all() and (u > 1e-12).any() and (u < -1e-12).any() and open_.float().mean() < 0.05
+    dy = torch.where(open_, torch.zeros_like(dy), dy)
+    _say("relu's side", shape, groups)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    y = ops.group_norm(leaves[0], groups, leaves[1], leaves[2], activation="relu")
+    assert ((y > 0) == (u > 0))[~open_].all()
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    # with the right slopes what is left are roundings: 64 of them of each term
+    du = torch.where(u > 0, dy.double(), torch.zeros_like(u))
+    g = du * w.double()
+    mean = lambda t: t.reshape(n, groups, -1).mean(dim=2, keepdim=True).expand(n, groups, c // groups).reshape(shape)  # noqa: E731
+    want = rstd * (g - mean(g) - hat * mean(g * hat))
+    size = rstd * (g.abs() + mean(g.abs()) + hat.abs() * mean((g * hat).abs()))
+    # xhat is off by the rounding of x - mean
+    ehat = 4 * U32 * (x.double().abs() * rstd + 1)
+    _within(dx, want, 64 * U32 * size + rstd * (ehat * mean((g * hat).abs()) + (hat.abs() + ehat) * mean(g.abs() * ehat)), "dx")
+    _within(db, du.sum(dim=(0, 1)), 64 * U32 * du.abs().sum(dim=(0, 1)) + 1e-38, "dbias")
+    _within(dw, (du * hat).sum(dim=(0, 1)), (du.abs() * (64 * U32 * hat.abs() + ehat)).sum(dim=(0, 1)) + 1e-38, "dweight")
