@@ -32,16 +32,20 @@ namespace {
 
 constexpr float kLog2e = 1.44269504088896341f;
 
-// exp(-v^2) P(1 / (1 + p v)), v >= 0: 1 - erf(v) within 1.5e-7 (Abramowitz and Stegun 7.1.26)
-__device__ __forceinline__ float erfc_pos(float v, float exp_v2) {
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, v, 1.f));
-  const float p = fmaf(fmaf(fmaf(fmaf(1.061405429f, t, -1.453152027f), t, 1.421413741f), t, -0.284496736f), t, 0.254829592f);
-  return p * t * exp_v2;
-}
-// the normal distribution's probability below u, and exp(-u^2 / 2)
+// The normal distribution's probability below u, and exp(-u^2 / 2).  Below -|u| it is exp(-u^2 / 2) t P(t) with
+// t = 1 / (1 + 0.3 |u| / sqrt 2): P is fitted to it by least squares reweighted towards the least
+// largest relative error, 2e-8 down to u = -14, so that gelu's negative tail, which is this alone, keeps its digits as
+// far as exp does.  Four terms fewer lose 2e-3 of it at -5, more than a rounding to float16, and save 2 % at most (20000 x
+// 13 x 1000, bfloat16, forward: 610 us for 621).
 __device__ __forceinline__ float normal_cdf(float u, float& e) {
   e = __builtin_amdgcn_exp2f(u * u * (-0.5f * kLog2e));
-  const float q = 0.5f * erfc_pos(fabsf(u) * 0.70710678118654752f, e);
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.212132034f, fabsf(u), 1.f));
+  float p = -0.06476129575f;
+  p = fmaf(p, t, 0.2427808618f), p = fmaf(p, t, -0.2561375458f);
+  p = fmaf(p, t, 0.273858342f), p = fmaf(p, t, -0.04732423627f);
+  p = fmaf(p, t, 0.1074625614f), p = fmaf(p, t, 0.07416970176f);
+  p = fmaf(p, t, 0.08535759755f), p = fmaf(p, t, 0.08459400352f);
+  const float q = p * t * e;
   return u < 0.f ? q : 1.f - q;
 }
 __device__ __forceinline__ float sigmoid(float u) {

@@ -4,7 +4,7 @@ from __future__ import annotations
 
 import pytest
 
-from tests.test_gpu_ops import DTYPES, U32, _check_norm, _norm64, _norm_case, _say, _within, _xent_case
+from tests.test_gpu_ops import DTYPES, HALF_ULP, TINY, U32, _check_norm, _norm64, _norm_case, _say, _within, _xent_case
 
 pytestmark = pytest.mark.gpu
 
@@ -295,3 +295,27 @@ def test_group_norm_relu_knows_its_side(gpu, shape, groups):
     _within(dx, want, 64 * U32 * size + rstd * (ehat * mean((g * hat).abs()) + (hat.abs() + ehat) * mean(g.abs() * ehat)), "dx")
     _within(db, du.sum(dim=(0, 1)), 64 * U32 * du.abs().sum(dim=(0, 1)) + 1e-38, "dbias")
     _within(dw, (du * hat).sum(dim=(0, 1)), (du.abs() * (64 * U32 * hat.abs() + ehat)).sum(dim=(0, 1)) + 1e-38, "dweight")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_group_norm_gelu_keeps_its_negative_tail(gpu, dtype):
+    """Weights of 0 make u the bias, exactly: gelu's value and slope from 0 to -9 to a relative error, where y comes down
+    to 1e-18.  exp's argument has three roundings (3 U32 u^2 / 2 of the result), the rest 40; the slope's two terms
+    count each.  Then the result's type."""
+    import torch
+    from mask_amd import ops
+    c = 4096
+    u = torch.linspace(-9.0, 3.0, c).cuda()
+    x = torch.randn(1, 1, c, generator=torch.Generator().manual_seed(61)).to(getattr(torch, dtype)).cuda()
+    w = torch.zeros(c, device="cuda")
+    b = u.clone().requires_grad_()
+    _say("gelu's tail", dtype)
+    y = ops.group_norm(x, 8, w, b, activation="gelu")
+    (db,) = torch.autograd.grad(y, b, torch.ones_like(y))
+    u = u.double()
+    cdf = 0.5 * torch.special.erfcx(u.abs() / 2 ** 0.5) * torch.exp(-0.5 * u * u)
+    cdf = torch.where(u < 0, cdf, 1 - cdf)
+    pdf = torch.exp(-0.5 * u * u) * 0.3989422804014327
+    rel = U32 * (1.5 * u * u + 40)
+    _within(y[0, 0], u * cdf, (u * cdf).abs() * (HALF_ULP[dtype] + rel) + TINY[dtype], "gelu")
+    _within(db, cdf + u * pdf, (cdf + (u * pdf).abs()) * (U32 + rel), "gelu's slope")
