@@ -146,50 +146,92 @@ __global__ __launch_bounds__(256) void k_few_layout(const T* __restrict__ f, int
   for (int i = 0; i < W; ++i) to[i * 64 + lane] = p[i];
 }
 
-// z[i][j][e]: row 16 i + 4 (lane / 16) + e of the short matrix with row[j] of the long one
-//
-// Loads return in order, so the order of their issue decides what runs under what: a step's short operands (from
-// L2), then the next step's rows (from memory), then the step's products, which
-// wait for the former only.
+// The short matrix's layout a line at a time, for all waves of a workgroup: a wave would fetch VT W KB of it from L2 for each
+// 2 TJ KB of its own rows, which bounded 65 and more short rows of 32 bits (60000 x 4096 against 100, float32: 702 us a
+// loss; 4 waves that share it take 423).  Lines pass through registers (`stage`), loaded a step before they are written,
+// to two places in LDS; one barrier a step.  Both layouts have as much a line.
+template <class T, int VT>
+struct Lines {
+  static constexpr int UNITS = Traits<T>::SUB * VT * Traits<T>::W, PER_WAVE = (UNITS + 3) / 4;   // of 1 KB
+  static_assert(UNITS == Traits<T>::OUT * (VT / 2) * Traits<T>::W, "the gradient's layout has the same lines");
+  typedef float4v Place[UNITS][64];
+  Place* lds;              // two
+  const float4v* from;
+  int count, lane, wave;
+  float4v stage[PER_WAVE];
+
+  __device__ __forceinline__ Lines(Place* lds_) : lds(lds_), lane(threadIdx.x & 63), wave(threadIdx.x >> 6) {}
+  __device__ __forceinline__ int unit(int k) const { return min(wave + 4 * k, UNITS - 1); }   // the last ones of some waves twice
+  __device__ __forceinline__ void fetch(int c) {
+    const float4v* p = from + (int64_t)min(c, count - 1) * (UNITS * 64) + lane;
+#pragma unroll
+    for (int k = 0; k < PER_WAVE; ++k) stage[k] = p[unit(k) * 64];
+  }
+  __device__ __forceinline__ void put(int c) {
+#pragma unroll
+    for (int k = 0; k < PER_WAVE; ++k) lds[c & 1][unit(k)][lane] = stage[k];
+  }
+  // all waves are done with the places' last use
+  __device__ __forceinline__ void begin(const float4v* layout, int lines) {
+    from = layout, count = lines;
+    fetch(0);
+    put(0);
+    fetch(1);
+  }
+  // Line c for all waves; its place is read until the next call.
+  __device__ __forceinline__ const Place& next(int c) {
+    barrier();
+    put(c + 1);
+    fetch(c + 2);
+    return lds[c & 1];
+  }
+  // LDS reads and writes before it are complete; loads stay in flight
+  static __device__ __forceinline__ void barrier() {
+    wait_lgkmcnt0();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  }
+};
+
+// z[i][j][e]: row 16 i + 4 (lane / 16) + e of the short matrix with row[j] of the long one.
+// All waves of the workgroup call it.
 template <class T, int VT, int TJ>
-__device__ __forceinline__ void logits(float4v (&z)[VT][TJ], const T* const (&row)[TJ], int dim, const float4v* fz, int lane) {
+__device__ __forceinline__ void logits(float4v (&z)[VT][TJ], const T* const (&row)[TJ], int dim, const float4v* fz,
+                                       Lines<T, VT>& lines) {
   constexpr int W = Traits<T>::W, KIND = Traits<T>::KIND, SUB = Traits<T>::SUB, LINE = Traits<T>::LINE;
 #pragma unroll
   for (int i = 0; i < VT; ++i)
 #pragma unroll
     for (int j = 0; j < TJ; ++j) z[i][j] = float4v{0.f, 0.f, 0.f, 0.f};
-  // lines in flight: a wave of 16 rows alone takes four to fill its share of the memory's latency
+  // lines of rows in flight: a wave of 16 rows alone takes four to fill its share of the memory's latency
   constexpr int PF = TJ == 1 ? 4 : 1;
-  const int q8 = 8 * (lane >> 4), whole = dim / LINE;
+  const int lane = lines.lane, q8 = 8 * (lane >> 4), whole = dim / LINE;
   Raw<T> next[PF][TJ];
   auto step = [&](int c, Raw<T> (&line)[TJ], bool more) {
-    float4v a[SUB][VT][W];
-    const float4v* p = fz + (int64_t)c * SUB * VT * W * 64 + lane;
-#pragma unroll
-    for (int s = 0; s < SUB; ++s)
-#pragma unroll
-      for (int i = 0; i < VT; ++i)
-#pragma unroll
-        for (int k = 0; k < W; ++k) a[s][i][k] = p[((s * VT + i) * W + k) * 64];
+    const auto& a_of = lines.next(c);
     Raw<T> cur[TJ];
 #pragma unroll
     for (int j = 0; j < TJ; ++j) cur[j] = line[j];
-    __builtin_amdgcn_sched_barrier(0);
     if (more)
 #pragma unroll
       for (int j = 0; j < TJ; ++j) load_line<T, false>(line[j], row[j], (c + PF) * LINE + q8, dim);
-    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_sched_barrier(0);   // loads first: they run under the products
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
       float4v b[TJ][W];
 #pragma unroll
       for (int j = 0; j < TJ; ++j) operand<T, W>(cur[j], s, b[j]);
 #pragma unroll
-      for (int i = 0; i < VT; ++i)
+      for (int i = 0; i < VT; ++i) {
+        float4v a[W];
 #pragma unroll
-        for (int j = 0; j < TJ; ++j) z[i][j] = mma_parts<KIND, W, W>(a[s][i], b[j], z[i][j]);
+        for (int k = 0; k < W; ++k) a[k] = a_of[(s * VT + i) * W + k][lane];
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) z[i][j] = mma_parts<KIND, W, W>(a, b[j], z[i][j]);
+      }
     }
   };
+  lines.begin(fz, (dim + LINE - 1) / LINE);
 #pragma unroll
   for (int u = 0; u < PF; ++u)
     if (u < whole)
@@ -227,11 +269,13 @@ __global__ __launch_bounds__(256) void k_few_loss(Args a, const float4v* __restr
                                                   float2* __restrict__ wave_sum) {
   const int lane = threadIdx.x & 63, wave = blockIdx.x * 4 + (threadIdx.x >> 6);
   const int t0 = wave * 16 * TJ;
-  if (t0 >= a.n_r) return;
   const T* row[TJ];
   row_pointers(row, a, t0, lane);
   float4v z[VT][TJ];
-  logits<T, VT, TJ>(z, row, a.dim, wz, lane);
+  __shared__ typename Lines<T, VT>::Place places[2];
+  Lines<T, VT> lines(places);
+  logits<T, VT, TJ>(z, row, a.dim, wz, lines);
+  if (t0 >= a.n_r) return;
   const int q4 = 4 * (lane >> 4);
   float sum = 0.f, count = 0.f;
 #pragma unroll
@@ -285,11 +329,13 @@ __global__ __launch_bounds__(256) void k_few_stats(Args a, const float4v* __rest
                                                    float* __restrict__ zt) {
   const int lane = threadIdx.x & 63, wave = blockIdx.x * 4 + (threadIdx.x >> 6);
   const int v0 = wave * 16 * TJ;
-  if (v0 >= a.n_r) return;
   const T* row[TJ];
   row_pointers(row, a, v0, lane);
   float4v z[VT][TJ];
-  logits<T, VT, TJ>(z, row, a.dim, fz, lane);
+  __shared__ typename Lines<T, VT>::Place places[2];
+  Lines<T, VT> lines(places);
+  logits<T, VT, TJ>(z, row, a.dim, fz, lines);
+  if (v0 >= a.n_r) return;
 #pragma unroll
   for (int i = 0; i < VT; ++i)
 #pragma unroll
@@ -326,11 +372,12 @@ __global__ __launch_bounds__(256, 2) void k_few_grad(Args a, const float4v* __re
   constexpr int W = Traits<T>::W, Z = Traits<T>::Z, KIND = Traits<T>::KIND;
   const int lane = threadIdx.x & 63, wave = blockIdx.x * 4 + (threadIdx.x >> 6);
   const int t0 = wave * 16 * TJ;
-  if (t0 >= pitch) return;   // waves past the last row fill dzt up to there
   const T* row[TJ];
-  row_pointers(row, a, t0, lane);
+  row_pointers(row, a, t0, lane);   // waves past the last row fill dzt up to `pitch`
   float4v z[VT][TJ];
-  logits<T, VT, TJ>(z, row, a.dim, wz, lane);
+  __shared__ typename Lines<T, VT>::Place places[2];
+  Lines<T, VT> lines(places);
+  logits<T, VT, TJ>(z, row, a.dim, wz, lines);
   const int q4 = 4 * (lane >> 4);
   const float unit = factor_unit(fmax);
   float4v b[VT / 2][TJ][Z];
@@ -387,29 +434,11 @@ __global__ __launch_bounds__(256, 2) void k_few_grad(Args a, const float4v* __re
   const float out = unit / Traits<T>::SCALE;
   constexpr int OUT = Traits<T>::OUT, LINE = Traits<T>::LINE;
   typedef T vec __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
-  const int lines = out_groups<T>(a.dim);
-  float4v next[OUT][VT / 2][W];
-  auto fetch = [&](int k) {
-    const float4v* p = wh + (int64_t)min(k, lines - 1) * OUT * (VT / 2) * W * 64 + lane;
-#pragma unroll
-    for (int o = 0; o < OUT; ++o)
-#pragma unroll
-      for (int c = 0; c < VT / 2; ++c)
-#pragma unroll
-        for (int i = 0; i < W; ++i) next[o][c][i] = p[((o * (VT / 2) + c) * W + i) * 64];
-  };
-  fetch(0);
-  for (int k = 0; k < lines; ++k) {
-    float4v w[OUT][VT / 2][W];
-#pragma unroll
-    for (int o = 0; o < OUT; ++o)
-#pragma unroll
-      for (int c = 0; c < VT / 2; ++c)
-#pragma unroll
-        for (int i = 0; i < W; ++i) w[o][c][i] = next[o][c][i];
-    __builtin_amdgcn_sched_barrier(0);
-    fetch(k + 1);
-    __builtin_amdgcn_sched_barrier(0);
+  const int n_lines = out_groups<T>(a.dim);
+  lines.barrier();   // the logits' last line is read
+  lines.begin(wh, n_lines);
+  for (int k = 0; k < n_lines; ++k) {
+    const auto& w_of = lines.next(k);
     const int d = LINE * k + 4 * OUT * (lane >> 4);   // this lane's 4 OUT features, 32 bytes
 #pragma unroll
     for (int j = 0; j < TJ; ++j) {
@@ -419,7 +448,12 @@ __global__ __launch_bounds__(256, 2) void k_few_grad(Args a, const float4v* __re
 #pragma unroll
       for (int c = 0; c < VT / 2; ++c)
 #pragma unroll
-        for (int o = 0; o < OUT; ++o) acc[o] = mma_parts<KIND, W, Z>(w[o][c], b[c][j], acc[o]);
+        for (int o = 0; o < OUT; ++o) {
+          float4v w[W];
+#pragma unroll
+          for (int i = 0; i < W; ++i) w[i] = w_of[(o * (VT / 2) + c) * W + i][lane];
+          acc[o] = mma_parts<KIND, W, Z>(w, b[c][j], acc[o]);
+        }
       const int t = t0 + 16 * j + (lane & 15);
       if (t >= a.n_r || d >= a.dim) continue;
       T* to = dh + (int64_t)t * a.dim + d;
@@ -550,8 +584,10 @@ void by_type(int dtype, F&& f) {
 }
 // 16-row tiles of the short matrix: 2, 4 or 8
 int short_tiles(int64_t n) { return n <= 32 ? 2 : n <= 64 ? 4 : 8; }
-// and of the long one a wave: 4 (with 128 short rows' dz in registers 2), or 1 where the waves would be few
-int long_tiles(int vt, int64_t n_r) { return n_r < 64 * 1024 ? 1 : vt == 8 ? 2 : 4; }
+// and of the long one a wave: 4 (with 128 short rows' dz in registers 2), or 1 where the waves would be few.
+// Training, float32, 2048 features: 120000 rows against 4 take 875 us for 1040 with one, 60000 532 for 510; 60000 against
+// 64 take 598 for 640, against 100 804 for 906, 40000 against 64 489 for 428.
+int long_tiles(int vt, int64_t n_r) { return n_r < (vt == 2 ? 64 : 48) * 1024 ? 1 : vt == 8 ? 2 : 4; }
 // 16-feature tiles of a workgroup of the short gradient
 template <class T>
 constexpr int short_columns(int vt) { return sizeof(T) == 2 && vt == 2 ? 8 : 4; }
@@ -603,12 +639,32 @@ struct Plan {
 
 }  // namespace few
 
-// Few rows of 16 bits that the general form's products can read where they are go
-// there in the forward pass: one row against 32000 classes of 2048 features takes 31 us for 40 here.
-bool few_forwards(const XentArgs& a, bool readable) {
-  return a.classes <= kFewClasses || (a.rows <= kFewRows && (a.dtype == kF32T || !readable));
+// Where this form is taken: it streams the long matrix, but each wave walks all features in turn, so a short long
+// matrix is faster in tiles, whose sums are split.  Times of the tiles are in brackets.
+namespace {
+// Few classes or rows, and a long matrix that fills the chip.  Training, float32, 4096 features: 5000 rows against 4 classes
+// take 254 us (264), 1500 245 (134); against 64 10000 335 (555), 5000 314 (295); against 100 20000 741 (1015), 10000 493 (598),
+// 5000 460 (312).  Few features are few steps, and packing the operands counts: 1500 x 256 against 4, float32, 52 us
+// (56), against 64 66 (61).
+bool is_few(const XentArgs& a) { return a.classes <= kFewClasses || a.rows <= kFewRows; }
+bool streams(const XentArgs& a) {
+  const bool by_rows = a.classes > kFewClasses;
+  const int vt = few::short_tiles(by_rows ? a.rows : a.classes);
+  if (a.dim < (vt == 2 ? 512 : vt == 4 ? 256 : 0)) return true;
+  return (by_rows ? a.classes : a.rows) >= (vt == 2 ? 4608 : vt == 4 ? 5632 : 12288);
 }
-bool few_backwards(const XentArgs& a) { return a.classes <= kFewClasses || a.rows <= kFewRows; }
+}  // namespace
+// 16 bits that the tiles' products can read where they are: the tiles copy nothing.  One row against 32000 classes of 2048
+// features: 40 us (31); float16, 60000 rows of 2048 against 100 classes 74 (49), 10000 against 4 30 (22), 60000 against 4 48 (55);
+// of up to 512 features both take a launch.
+bool few_forwards(const XentArgs& a, bool readable) {
+  if (!is_few(a)) return false;
+  if (a.dtype == kF32T) return streams(a);
+  if (!readable) return a.dim < 1024 || streams(a);
+  return a.classes <= kFewClasses && (a.dim < 1024 || (a.classes <= 32 && a.rows >= 20000));
+}
+// In 16 bits this form's dz has two parts, the tiles' one.
+bool few_backwards(const XentArgs& a) { return is_few(a) && (a.dtype != kF32T || streams(a)); }
 
 size_t few_forward(const XentArgs& a, float* loss, hipStream_t s) {
   using namespace few;
@@ -663,9 +719,7 @@ size_t few_backward(const XentArgs& a, const float* dloss, void* dh, void* dw, h
     by_tiles(p.vt, [&](auto vt) {
       constexpr int VT = decltype(vt)::value;
       by_long<VT>(p.tj, [&](auto tj) {
-        // six parts of 128 short rows' dz leave registers for one tile only (100000 x 256 against 100, float32,
-        // forward and backward: 318 us for 367 with two)
-        constexpr int TJ = sizeof(T) == 4 && VT == 8 ? 1 : decltype(tj)::value;
+        constexpr int TJ = decltype(tj)::value;
         auto* k = by_rows ? k_few_grad<T, VT, TJ, true> : k_few_grad<T, VT, TJ, false>;
         k<<<(unsigned)((pitch + 64 * TJ - 1) / (64 * TJ)), 256, 0, s>>>(p.args, p.wz, p.wh, factor, fmax, dzt, pitch, (T*)dlong);
       });

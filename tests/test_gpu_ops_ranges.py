@@ -4,7 +4,7 @@ from __future__ import annotations
 
 import pytest
 
-from tests.test_gpu_ops import DTYPES, HALF_ULP, TINY, U32, _check_norm, _norm64, _norm_case, _say, _within, _xent_case
+from tests.test_gpu_ops import DTYPES, HALF_ULP, TINY, U32, _check_norm, _check_xent, _norm64, _norm_case, _say, _within, _xent_case
 
 pytestmark = pytest.mark.gpu
 
@@ -319,3 +319,18 @@ def test_group_norm_gelu_keeps_its_negative_tail(gpu, dtype):
     rel = U32 * (1.5 * u * u + 40)
     _within(y[0, 0], u * cdf, (u * cdf).abs() * (HALF_ULP[dtype] + rel) + TINY[dtype], "gelu")
     _within(db, cdf + u * pdf, (cdf + (u * pdf).abs()) * (U32 + rel), "gelu's slope")
+
+
+# ---- where the forms of the cross entropy change -----------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(4607, 520, 9), (4608, 520, 9), (1000, 511, 9), (5631, 260, 40), (5632, 260, 40), (1000, 255, 40),
+                                   (12287, 70, 100), (12288, 70, 100), (9, 520, 4607), (9, 520, 4608), (40, 260, 5632),
+                                   (100, 70, 12287), (100, 70, 12288), (49152, 24, 64), (49151, 24, 64), (65536, 24, 9),
+                                   (70, 1024, 90), (70, 1025, 90), (20000, 1024, 20), (19999, 1024, 20)])
+def test_linear_cross_entropy_where_its_forms_change(gpu, shape, dtype):
+    """On both sides of the sizes from which the long matrix is streamed, of the features from which it counts, and of
+    the tiles of a wave; workgroups whose last waves have no rows."""
+    _say("forms", shape, dtype)
+    h, w, t = _xent_case(*shape, dtype, seed=71)
+    _check_xent(h, w, t, "mean", what=f"{shape} {dtype}")
