@@ -17,8 +17,8 @@
 // relu's slope jumps at u = 0, so a rounding of u there switches whole
 // gradient entries (one of 60 million channels of nodes is 5e-4 of its weight's gradient). Mean, rstd and rstd w are
 // therefore kept as two floats each, and relu's u is summed from both, in the forward and the backward pass
-// alike: what decides its sign is the statistics' own error.  Of single float32 rows, summed in 64 bits, that is
-// about 1e-14.  In the other forms, and in 16 bits, a thread adds its values in 32 bits: the mean is off by up to
+// alike: what decides its sign is the statistics' own error.  Of float32 samples of one row, or of few (a thread has one),
+// summed in 64 bits, that is about 1e-14.  In the others, and in 16 bits, a thread adds its values in 32 bits: the mean is off by up to
 // 2^-24 of them and the variance by 2^-24 of itself a value that a thread adds, mostly far less, as the threads'
 // errors are of either sign.  It costs no time: the passes wait for memory.
 #include <hip/hip_runtime.h>
@@ -210,9 +210,9 @@ struct Small {
 // Sums of `v` over each group of each of the workgroup's samples: end(i, sums) in one
 // thread for i = sample * groups + group.  All threads of the workgroup call it, and
 // what `end` leaves in LDS is there for all afterwards.
-template <int V, int N, class F>
+template <int V, int N, class R, class F>
 __device__ __forceinline__ void group_sums(const Shape& sh, const Small& sm, bool on, int s, int rt, int cv,
-                                           float (&v)[N][V], float* red, F&& end) {
+                                           R (&v)[N][V], R* red, F&& end) {
   const bool whole = sh.per_group % V == 0;   // a vector lies in one group
   const int width = whole ? sm.vectors : sh.channels, per = whole ? sh.per_group / V : sh.per_group;
   const int slice = sm.samples * sm.row_threads * width, ns = sm.samples * sh.groups;
@@ -221,7 +221,7 @@ __device__ __forceinline__ void group_sums(const Shape& sh, const Small& sm, boo
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       if (whole) {
-        float t = v[k][0];
+        R t = v[k][0];
 #pragma unroll
         for (int e = 1; e < V; ++e) t += v[k][e];
         red[k * slice + at + cv] = t;
@@ -242,7 +242,7 @@ __device__ __forceinline__ void group_sums(const Shape& sh, const Small& sm, boo
     for (int k = 0; k < N; ++k) t[k] = 0.;
     if (i < ns) {
       const int si = i / sh.groups, g = i - si * sh.groups;
-      const float* in = red + si * sm.row_threads * width + g * per;
+      const R* in = red + si * sm.row_threads * width + g * per;
       for (int r = r0, j = j0; r < sm.row_threads;) {
 #pragma unroll
         for (int k = 0; k < N; ++k) t[k] += in[k * slice + r * width + j];
@@ -270,12 +270,20 @@ __device__ __forceinline__ void of_groups(P (&to)[V], const P* from, const int (
   }
 }
 
+// threads of a workgroup at most: single channels a thread leave registers for twice as many
+__host__ __device__ constexpr int small_threads(int v) { return v == 1 ? 1024 : 512; }
+
+// A thread's sums of the statistics: 64 bits where a thread has one row of 32 bits, for relu's side
+template <class T, int NR>
+using SmallSum = std::conditional_t<sizeof(T) == 4 && NR == 1, double, float>;
+
 template <class T, int V, int NR>
-__global__ __launch_bounds__(512) void k_norm_small(Shape sh, Small sm, const T* __restrict__ x, T* __restrict__ y,
+__global__ __launch_bounds__(small_threads(V)) void k_norm_small(Shape sh, Small sm, const T* __restrict__ x, T* __restrict__ y,
                                                      float4* __restrict__ stats) {
   extern __shared__ double sums[];   // of each group of each sample the mean and its statistics, then the threads' sums
   float4* st = (float4*)(sums + ((sm.samples * sh.groups + 1) & ~1));
-  float* red = (float*)(st + sm.samples * sh.groups);
+  using R = SmallSum<T, NR>;
+  R* red = (R*)(st + sm.samples * sh.groups);
   const int per_sample = sm.row_threads * sm.vectors;
   const int s = threadIdx.x / per_sample, u = threadIdx.x - s * per_sample, rt = u / sm.vectors, cv = u - rt * sm.vectors;
   const int c0 = cv * V;
@@ -296,9 +304,9 @@ __global__ __launch_bounds__(512) void k_norm_small(Shape sh, Small sm, const T*
     for (int i = 0; i < NR; ++i)
       if (on && rt + i * sm.row_threads < sh.length)
         raw[i] = *(const Vec<T, V>*)(xs + (rt + i * sm.row_threads) * sh.ldx);
-    float t[1][V];
+    R t[1][V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) t[0][e] = 0.f;
+    for (int e = 0; e < V; ++e) t[0][e] = 0;
     if (on)
 #pragma unroll
       for (int i = 0; i < NR; ++i)
@@ -312,16 +320,16 @@ __global__ __launch_bounds__(512) void k_norm_small(Shape sh, Small sm, const T*
     if (on) {
       double mean64[V];
       of_groups<V>(mean64, sums, g, whole);
-      float mean[V];
+      R mean[V];
 #pragma unroll
-      for (int e = 0; e < V; ++e) mean[e] = (float)mean64[e], t[0][e] = 0.f;
+      for (int e = 0; e < V; ++e) mean[e] = (R)mean64[e], t[0][e] = 0;
 #pragma unroll
       for (int i = 0; i < NR; ++i)
         if (rt + i * sm.row_threads < sh.length) {
           float f[V];
           widen<T, V>(raw[i], f);
 #pragma unroll
-          for (int e = 0; e < V; ++e) t[0][e] = fmaf(f[e] - mean[e], f[e] - mean[e], t[0][e]);
+          for (int e = 0; e < V; ++e) t[0][e] = fma(f[e] - mean[e], f[e] - mean[e], t[0][e]);
         }
     }
     group_sums<V, 1>(sh, sm, on, s, rt, cv, t, red, [&](int i, const double(&v)[1]) {
@@ -370,7 +378,7 @@ __device__ __forceinline__ void join_params(const Shape& sh, int rows, const flo
 }
 
 template <class T, int V, int NR>
-__global__ __launch_bounds__(512) void k_norm_small_bwd(Shape sh, Small sm, const T* __restrict__ x,
+__global__ __launch_bounds__(small_threads(V)) void k_norm_small_bwd(Shape sh, Small sm, const T* __restrict__ x,
                                                          const T* __restrict__ dy, T* __restrict__ dx,
                                                          const float4* __restrict__ stats, float2* __restrict__ part) {
   extern __shared__ double sums[];   // of each group of each sample two means, then the threads' sums
@@ -1100,11 +1108,12 @@ struct SmallPlan {
 };
 
 // A sample in one workgroup, up to 8 vectors a thread.  Few long samples
-// would leave most CUs without work: they are split instead.
+// would leave most CUs without work: they are split instead.  Split short samples are parts of one row each: 58809 rows
+// of 728 channels in groups of 91, bfloat16, which have one channel a thread, took 1097 us so, and take 154 (training 16418 and 315).
 SmallPlan small_plan(const NormArgs& a, int v) {
   SmallPlan p;
   const int64_t cv = a.channels / v, vectors = a.length * cv;
-  if (cv > 512 || (a.batch < 64 && vectors > 1024 * 2)) return p;
+  if (a.batch < 64 && vectors > 1024 * 2) return p;
   const int64_t cg = a.channels / a.groups;
   if (a.length == 1 && cg % v == 0) {
     int lanes = 1, w = 1;
@@ -1124,8 +1133,8 @@ SmallPlan small_plan(const NormArgs& a, int v) {
       return p;
     }
   }
-  for (int t : {256, 512}) {
-    if (cv > t) continue;
+  for (int t = 256; t <= small_threads(v); t *= 2) {
+    if (cv > t || (t == 1024 && cv <= 512)) continue;
     const int64_t rt = t / cv < a.length ? t / cv : a.length, nr = (a.length + rt - 1) / rt;
     int64_t samples = t / (rt * cv);
     if (samples > a.batch) samples = a.batch;
@@ -1250,7 +1259,8 @@ void norm_forward(const NormArgs& a, void* y, hipStream_t s) {
   const Shape sh = shape_of(a, 0, 0);
   Carver c(a.ws);
   if (sp.ok) {
-    const size_t lds = sp.sm.samples * (sp.sm.row_threads * sp.sm.vectors * v * sizeof(float) + a.groups * (sizeof(float4) + sizeof(double))) + sizeof(double);
+    const size_t sum = a.dtype == kF32T && sp.nr == 1 ? sizeof(double) : sizeof(float);   // SmallSum
+    const size_t lds = sp.sm.samples * (sp.sm.row_threads * sp.sm.vectors * v * sum + a.groups * (sizeof(float4) + sizeof(double))) + sizeof(double);
     by_type(a.dtype, [&](auto* t) {
       using T = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
       by_vector<T>(v, [&](auto vc) {

@@ -334,3 +334,13 @@ def test_linear_cross_entropy_where_its_forms_change(gpu, shape, dtype):
     _say("forms", shape, dtype)
     h, w, t = _xent_case(*shape, dtype, seed=71)
     _check_xent(h, w, t, "mean", what=f"{shape} {dtype}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape, groups", [((90, 1, 728), 8), ((70, 1, 1023), 1), ((70, 1, 1023), 3), ((80, 1, 992), 32), ((66, 1, 1025), 5),
+                                           ((70, 3, 1023), 1), ((65, 7, 777), 7), ((600, 1, 1024), 1024), ((70, 9, 1001), 1001)])
+def test_group_norm_of_many_odd_channels(gpu, shape, groups, dtype):
+    """More than 512 channels that no vector divides: a channel a thread, up to 1024 of them, and one more."""
+    x, w, b, dy = _norm_case(shape, groups, "gelu", dtype, seed=42)
+    _say("odd channels", shape, groups, dtype)
+    _check_norm(x, groups, w, b, dy, "gelu", what=f"{shape} {groups} {dtype}")
