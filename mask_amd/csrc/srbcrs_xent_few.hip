@@ -476,8 +476,9 @@ __global__ __launch_bounds__(256, 2) void k_few_grad(Args a, const float4v* __re
 }
 
 // Part of the short matrix's gradient: the long one's rows in steps of 32, dealt to the waves of all of
-// a part's workgroups; 16 NJ features a workgroup.  Lane's features of tile j: d0 + NJ (lane % 16) + j, so that it
-// loads NJ next to each other.  dz^T is read once for all of a workgroup's features: NJ is 8 where
+// a part's workgroups; 16 NJ features a workgroup.  A lane's features of tile j: d0 + APART j, in 16 bits next to each other
+// and loaded together, in 32 each by itself: 16 bytes a lane of rows that are not aligned to them come at half the rate (81064 x
+// 3126 against 10: 480 us for 265), and of rows that are no faster.  dz^T is read once for all of a workgroup's features: NJ is 8 where
 // registers allow.  A long row of factor 0 (null: all are 1) counts as zeros whatever it holds.
 template <class T, int VT, int NJ>
 __global__ __launch_bounds__(256, VT * NJ >= 32 ? 1 : 2) void k_few_short(Args a, const float* __restrict__ factor, const float* __restrict__ dzt,
@@ -485,7 +486,8 @@ __global__ __launch_bounds__(256, VT * NJ >= 32 ? 1 : 2) void k_few_short(Args a
   constexpr int W = Traits<T>::W, Z = Traits<T>::Z, KIND = Traits<T>::KIND;
   __shared__ float sum[VT * 16 * 16 * NJ];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q8 = 8 * (lane >> 4);
-  const int d0 = (blockIdx.x * 16 + r) * NJ;
+  constexpr int APART = sizeof(T) == 4 ? 16 : 1;
+  const int d0 = blockIdx.x * 16 * NJ + (APART == 1 ? NJ * r : r);
   typedef T vecn __attribute__((ext_vector_type(NJ), aligned(sizeof(T))));
   float4v acc[VT][NJ];
 #pragma unroll
@@ -493,7 +495,7 @@ __global__ __launch_bounds__(256, VT * NJ >= 32 ? 1 : 2) void k_few_short(Args a
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[i][j] = float4v{0.f, 0.f, 0.f, 0.f};
   const int64_t steps = pitch / 32;
-  const bool whole = d0 + NJ <= a.dim;
+  const bool whole = d0 + APART * (NJ - 1) < a.dim;
   vecn raw[8];
   float4v f[2], zraw[VT][2];
   // a step's values; dzt and factor reach to whole steps, h is read at its last row past the end
@@ -509,10 +511,10 @@ __global__ __launch_bounds__(256, VT * NJ >= 32 ? 1 : 2) void k_few_short(Args a
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const T* p = (const T*)a.r + min(t0 + e, (int64_t)a.n_r - 1) * a.ld + d0;
-      if (whole) raw[e] = *(const vecn*)p;
+      if (APART == 1 && whole) raw[e] = *(const vecn*)p;
       else
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) raw[e][j] = d0 + j < a.dim ? p[j] : (T)0.f;
+        for (int j = 0; j < NJ; ++j) raw[e][j] = whole || d0 + APART * j < a.dim ? p[APART * j] : (T)0.f;
     }
 #pragma unroll
     for (int i = 0; i < VT; ++i) {
@@ -564,7 +566,7 @@ __global__ __launch_bounds__(256, VT * NJ >= 32 ? 1 : 2) void k_few_short(Args a
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float* p = sum + (16 * i + 4 * (lane >> 4) + e) * (16 * NJ) + NJ * r + j;
+            float* p = sum + (16 * i + 4 * (lane >> 4) + e) * (16 * NJ) + d0 - blockIdx.x * 16 * NJ + APART * j;
             *p = w ? *p + acc[i][j][e] : acc[i][j][e];
           }
     __syncthreads();
