@@ -494,6 +494,9 @@ int srbcrs_group_norm_backward(const srbcrs_norm_desc *desc, const void *d_dy, c
  * weight classes x dim, both of `dtype`.  A row whose target is ignore_index
  * has a loss of 0, does not count in the mean and gets a gradient of 0; a
  * target outside [0, classes) that is not ignore_index gives a loss of NaN.
+ * 32-bit values keep 22 bits (24 with few classes or rows) in the products, of
+ * each row of h and of the weight to its own largest value in the logits, to the
+ * largest of all that count in the gradients' sums; 16-bit ones are used as they are.
  * reduction: NONE writes `rows` floats to d_loss, MEAN (over the labelled
  * rows; 0 if there is none) and SUM one.  d_state, 2 * rows + 1 floats (8-byte
  * aligned), is kept from the forward pass for the backward pass. */

@@ -198,7 +198,7 @@ struct Affine {
 // ---- a sample in one workgroup's registers ----------------------------------
 //
 // x (and dy) are read once; what bounds it is the wait for the other threads, twice forward and once backward.
-// 20000 x 5 x 96 in 8 groups, float32, relu: 30 us forward (2.6 TB/s), 35 backward (3.3).
+// 20000 x 5 x 96 in 8 groups, float32, relu: 31 us forward (2.5 TB/s), 37 backward (3.1).
 
 struct Small {
   int row_threads;   // threads along a sample's rows
@@ -507,7 +507,7 @@ struct RowPlace {
 // A thread keeps its channels and walks samples, 4 / W in flight; nothing is shared
 // beyond the wave, so no wave waits for another.  Sums of 32-bit features are 64 bits
 // from the start, as relu's side asks for; of 16-bit ones 32 bits.  Memory bounds it: 65536 x 512 in 8
-// groups, float32, gelu: 60 us, 4440 GB/s; with the sums through LDS it took 133.
+// groups, float32, gelu: 66 us, 4080 GB/s; with the sums through LDS it took 133.
 template <class T, int V, int W>
 __global__ __launch_bounds__(512) void k_norm_rows(Shape sh, Small sm, const T* __restrict__ x, T* __restrict__ y,
                                                     float4* __restrict__ stats) {
@@ -635,7 +635,7 @@ __global__ __launch_bounds__(512) void k_norm_rows_bwd(Shape sh, Small sm, const
 // ---- a sample split along its rows ------------------------------------------
 //
 // Four passes over memory, which bounds each.  One sample of 232965 x 256 in 32 groups, float32, relu:
-// statistics 49 us (4.9 TB/s), y 73 (6.5, some of x from the last-level cache), sums of the gradient 80 (6.0), dx 141 (5.1).
+// statistics 48 us (5.0 TB/s), y 74 (6.4, some of x from the last-level cache), sums of the gradient 83 (5.8), dx 142 (5.0).
 
 struct Chunks {
   int row_threads, vectors;   // threads of a workgroup along rows and channels

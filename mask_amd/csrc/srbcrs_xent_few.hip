@@ -1,12 +1,12 @@
 // Linear cross entropy where one of its two matrices has few rows: few classes
 // (a graph network's classifier) or few rows of features (tokens to score
 // against a large vocabulary).  The other matrix is read where it is, once a
-// product, and that is what bounds it.
+// product, and that is what bounds it where it is long (streams, below).
 //
 // A wave holds the logits of its rows of the long matrix with all rows of the short one in
-// registers.  The matrix instructions' operands come straight from memory: a
-// lane's 8 values of a long row are next to each other there, and the short matrix is laid
-// out once a call in the order in which the lanes take it (it stays in L2).  dz
+// registers.  The matrix instructions' operands of the long one come straight from memory: a
+// lane's 8 values of a row are next to each other there.  The short matrix is laid
+// out once a call in the order in which the lanes take it, and comes to LDS a line at a time for the workgroup.  dz
 // leaves the logits' registers as the operand of the next product: the
 // short dimension is summed in the order in which the registers hold it, on both sides.
 //
@@ -19,8 +19,9 @@
 // 32-bit values are three bfloat16 (24 bits, no scale needed), six products; dz of
 // 16-bit inputs is two of their type.  Sums are 32 bits.
 //
-// 232965 rows of 256 features against 64 classes, float32: loss 69 us (3.5 TB/s), dz and
-// dh 158 (3.4 TB/s), dw 95 (3.1); the products take a third to a half of it and mostly run under the loads.
+// 232965 rows of 256 features against 64 classes, float32: loss 64 us (3.7 TB/s), dz and
+// dh 143 (3.3 TB/s), dw 98 (3.0); the products take a third to a half of it and mostly run under the loads.
+// Rows that are not aligned to 16 bytes are read and written at two thirds of that.
 #include <hip/hip_runtime.h>
 
 #include "srbcrs_xent.hpp"
@@ -644,11 +645,11 @@ struct Plan {
 // Where this form is taken: it streams the long matrix, but each wave walks all features in turn, so a short long
 // matrix is faster in tiles, whose sums are split.  Times of the tiles are in brackets.
 namespace {
+bool is_few(const XentArgs& a) { return a.classes <= kFewClasses || a.rows <= kFewRows; }
 // Few classes or rows, and a long matrix that fills the chip.  Training, float32, 4096 features: 5000 rows against 4 classes
 // take 254 us (264), 1500 245 (134); against 64 10000 335 (555), 5000 314 (295); against 100 20000 741 (1015), 10000 493 (598),
 // 5000 460 (312).  Few features are few steps, and packing the operands counts: 1500 x 256 against 4, float32, 52 us
 // (56), against 64 66 (61).
-bool is_few(const XentArgs& a) { return a.classes <= kFewClasses || a.rows <= kFewRows; }
 bool streams(const XentArgs& a) {
   const bool by_rows = a.classes > kFewClasses;
   const int vt = few::short_tiles(by_rows ? a.rows : a.classes);
